@@ -1,0 +1,177 @@
+// C ABI of the optimizer operators (AdamW step, gradient norm): argument checks, tables and launches.  The entry points are
+// documented in include/gcn_uelb_hip.h.
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/gcn_uelb_hip.h"
+#include "host.hpp"
+#include "kernels_optim.hpp"
+
+namespace {
+
+constexpr int kAdamwUnits = 2;       // 2048-element strides of a workgroup of k_adamw
+
+size_t elem_size(int type) { return type == GCN_F32 ? 4 : 2; }
+
+bool aligned_to(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
+uint64_t units_of(uint64_t n, uint64_t unit) { return (n + unit - 1) / unit; }
+
+// strides of a workgroup of k_grad_norm: enough workgroups to fill the chip, few enough partial sums for one workgroup to add
+int norm_units(uint64_t total) { return total <= (1ull << 24) ? 2 : total <= (1ull << 28) ? 16 : 64; }
+
+int check_numel(const char* who, int n, const long long* numel, uint64_t* total) {
+    *total = 0;
+    for (int k = 0; k < n; ++k) {
+        if (numel[k] < 0 || numel[k] >= (1ll << 40)) return fail(-1, "%s: tensor %d has %lld elements", who, k, numel[k]);
+        *total += (uint64_t)numel[k];
+    }
+    if (*total >= (1ull << 42)) return fail(-2, "%s: %llu elements in all", who, (unsigned long long)*total);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gcn_adamw_hyper_bytes(void) { return sizeof(AdamwHyper); }
+
+static int check_adamw(const gcn_adamw_desc* d) {
+    if (!d) return fail(-1, "gcn_adamw: null descriptor");
+    if (d->n < 0) return fail(-1, "gcn_adamw: n = %d", d->n);
+    if (d->param_type < GCN_F32 || d->param_type > GCN_F16) return fail(-1, "gcn_adamw: unknown parameter type %d", d->param_type);
+    if (d->state_bits != 32 && d->state_bits != 8) return fail(-1, "gcn_adamw: states of %d bits (32 or 8)", d->state_bits);
+    if (!(d->lr >= 0.0) || !(d->eps >= 0.0) || !(d->weight_decay >= 0.0)) return fail(-1, "gcn_adamw: negative lr, eps or weight_decay");
+    if (!(d->beta1 >= 0.0 && d->beta1 < 1.0) || !(d->beta2 >= 0.0 && d->beta2 < 1.0)) return fail(-1, "gcn_adamw: betas outside [0, 1)");
+    return 0;
+}
+
+int gcn_adamw_advance(const gcn_adamw_desc* d, long long* step, const float* lr, void* hyper, void* stream) {
+    if (int rc = check_adamw(d)) return rc;
+    if (!step || !hyper) return fail(-1, "gcn_adamw_advance: null pointer argument");
+    if (!aligned_to(step, 8) || !aligned_to(hyper, 8)) return fail(-1, "gcn_adamw_advance: pointer not aligned to 8 bytes");
+    hipStream_t st = (hipStream_t)stream;
+    GCN_PROF_PRE("k_adamw_advance");
+    k_adamw_advance<<<1, 1, 0, st>>>(step, lr, (AdamwHyper*)hyper, d->lr, d->beta1, d->beta2, d->eps, d->weight_decay, d->seed);
+    GCN_CHECK_LAUNCH("k_adamw_advance");
+    return 0;
+}
+
+int gcn_adamw_step(const gcn_adamw_desc* d, void* const* params, const void* const* grads, float* const* masters, void* const* exp_avg,
+                   void* const* exp_avg_sq, unsigned char* const* exp_avg_exp, unsigned char* const* exp_avg_sq_exp, const long long* numel,
+                   const float* grad_scale, const float* clip_coef, const void* hyper, void* stream) {
+    if (int rc = check_adamw(d)) return rc;
+    const bool eight = d->state_bits == 8, half = d->param_type != GCN_F32;
+    if (!hyper && d->step < 1) return fail(-1, "gcn_adamw_step: step %lld < 1", d->step);
+    if (d->n > 0 && (!params || !grads || !exp_avg || !exp_avg_sq || !numel)) return fail(-1, "gcn_adamw_step: null pointer argument");
+    if (d->n > 0 && half != (masters != nullptr)) return fail(-1, "gcn_adamw_step: master copies go with 16-bit parameters, and only with them");
+    if (d->n > 0 && eight != (exp_avg_exp != nullptr && exp_avg_sq_exp != nullptr)) return fail(-1, "gcn_adamw_step: exponent bytes go with 8-bit states, and only with them");
+    uint64_t total;
+    if (int rc = check_numel("gcn_adamw_step", d->n, numel, &total)) return rc;
+    const size_t pe = elem_size(d->param_type), se = eight ? 1 : 4;
+    for (int k = 0; k < d->n; ++k) {
+        if (numel[k] == 0) continue;
+        if (!params[k] || !grads[k] || !exp_avg[k] || !exp_avg_sq[k] || (half && !masters[k]) || (eight && (!exp_avg_exp[k] || !exp_avg_sq_exp[k])))
+            return fail(-1, "gcn_adamw_step: tensor %d has a null pointer", k);
+        if (!aligned_to(params[k], pe) || !aligned_to(grads[k], pe) || !aligned_to(exp_avg[k], se) || !aligned_to(exp_avg_sq[k], se) ||
+            (half && !aligned_to(masters[k], 4)))
+            return fail(-1, "gcn_adamw_step: tensor %d is not aligned to its elements", k);
+    }
+    hipStream_t st = (hipStream_t)stream;
+    const AdamwHyper h = hyper ? AdamwHyper{} : opt_hyper(d->lr, d->beta1, d->beta2, d->eps, d->weight_decay, d->step, d->seed);
+    OptTable t;
+    t.stride = 5 + (half ? 1 : 0) + (eight ? 2 : 0);
+    const int most = std::min(OPT_MAX_TENSORS, OPT_WORDS / t.stride);
+    for (int k = 0; k < d->n;) {
+        t.n = 0;
+        t.ordinal = d->first_tensor + (uint32_t)k;
+        uint64_t blocks = 0;
+        // tensors keep their numbers: an empty one takes a place without workgroups
+        for (; k < d->n && t.n < most; ++k, ++t.n) {
+            const uint64_t more = units_of((uint64_t)numel[k], kAdamwUnits * OPT_STRIDE);
+            if (blocks + more > 0x7fffffffull) {
+                if (t.n == 0) return fail(-2, "gcn_adamw_step: tensor %d is too large for one launch", k);
+                break;
+            }
+            uint64_t* w = t.w + (size_t)t.n * t.stride;
+            bool vec = aligned_to(params[k], 16) && aligned_to(grads[k], 16) && aligned_to(exp_avg[k], eight ? 8 : 16) && aligned_to(exp_avg_sq[k], eight ? 8 : 16);
+            if (half) vec = vec && aligned_to(masters[k], 16);
+            w[0] = (uint64_t)numel[k] | (vec ? OPT_VEC : 0);
+            w[1] = (uint64_t)params[k]; w[2] = (uint64_t)grads[k]; w[3] = (uint64_t)exp_avg[k]; w[4] = (uint64_t)exp_avg_sq[k];
+            int at = 5;
+            if (half) w[at++] = (uint64_t)masters[k];
+            if (eight) { w[at++] = (uint64_t)exp_avg_exp[k]; w[at] = (uint64_t)exp_avg_sq_exp[k]; }
+            t.first[t.n] = (uint32_t)blocks;
+            blocks += more;
+        }
+        if (blocks == 0) continue;
+        GCN_PROF_PRE("k_adamw");
+#define ADAMW_LAUNCH(P, M, E) k_adamw<kAdamwUnits, P, M, E><<<(uint32_t)blocks, OPT_THREADS, 0, st>>>(t, h, (const AdamwHyper*)hyper, grad_scale, clip_coef)
+        if (d->param_type == GCN_F32) { if (eight) ADAMW_LAUNCH(float, false, true); else ADAMW_LAUNCH(float, false, false); }
+        else if (d->param_type == GCN_BF16) { if (eight) ADAMW_LAUNCH(__bf16, true, true); else ADAMW_LAUNCH(__bf16, true, false); }
+        else { if (eight) ADAMW_LAUNCH(_Float16, true, true); else ADAMW_LAUNCH(_Float16, true, false); }
+#undef ADAMW_LAUNCH
+        GCN_CHECK_LAUNCH("k_adamw");
+    }
+    return 0;
+}
+
+size_t gcn_grad_norm_ws_bytes(int n, const long long* numel) {
+    uint64_t total = 0, blocks = 0;
+    if (n < 0 || (n > 0 && !numel) || check_numel("gcn_grad_norm_ws_bytes", n, numel, &total)) return 0;
+    const int units = norm_units(total);
+    for (int k = 0; k < n; ++k) blocks += units_of((uint64_t)numel[k], (uint64_t)units * OPT_STRIDE);
+    return std::max<size_t>(blocks, 1) * sizeof(double);
+}
+
+int gcn_grad_norm(int n, int type, const void* const* grads, const long long* numel, const float* grad_scale, double max_norm, float* out,
+                  void* ws, size_t ws_bytes, void* stream) {
+    if (n < 0 || (n > 0 && (!grads || !numel)) || !out) return fail(-1, "gcn_grad_norm: null pointer argument or n = %d", n);
+    if (type < GCN_F32 || type > GCN_F16) return fail(-1, "gcn_grad_norm: unknown type %d", type);
+    if (!(max_norm >= 0.0)) return fail(-1, "gcn_grad_norm: max_norm %g", max_norm);
+    uint64_t total;
+    if (int rc = check_numel("gcn_grad_norm", n, numel, &total)) return rc;
+    for (int k = 0; k < n; ++k)
+        if (numel[k] > 0 && (!grads[k] || !aligned_to(grads[k], elem_size(type)))) return fail(-1, "gcn_grad_norm: tensor %d has a null or misaligned pointer", k);
+    if (!ws || !aligned_to(ws, 8) || ws_bytes < gcn_grad_norm_ws_bytes(n, numel)) return fail(-2, "gcn_grad_norm: workspace too small");
+    hipStream_t st = (hipStream_t)stream;
+    const int units = norm_units(total);
+    double* part = (double*)ws;
+    uint64_t done = 0;
+    OptTable t;
+    t.stride = 2;
+    t.ordinal = 0;
+    for (int k = 0; k < n;) {
+        t.n = 0;
+        uint64_t blocks = 0;
+        for (; k < n && t.n < OPT_MAX_TENSORS; ++k, ++t.n) {
+            const uint64_t more = units_of((uint64_t)numel[k], (uint64_t)units * OPT_STRIDE);
+            if (blocks + more > 0x7fffffffull) {
+                if (t.n == 0) return fail(-2, "gcn_grad_norm: tensor %d is too large for one launch", k);
+                break;
+            }
+            t.w[2 * t.n] = (uint64_t)numel[k] | (aligned_to(grads[k], 16) ? OPT_VEC : 0);
+            t.w[2 * t.n + 1] = (uint64_t)grads[k];
+            t.first[t.n] = (uint32_t)blocks;
+            blocks += more;
+        }
+        if (blocks == 0) continue;
+        GCN_PROF_PRE("k_grad_norm");
+#define NORM_LAUNCH(U, P) k_grad_norm<U, P><<<(uint32_t)blocks, OPT_THREADS, 0, st>>>(t, part + done)
+#define NORM_LAUNCH_T(P) do { if (units == 2) NORM_LAUNCH(2, P); else if (units == 16) NORM_LAUNCH(16, P); else NORM_LAUNCH(64, P); } while (0)
+        if (type == GCN_F32) NORM_LAUNCH_T(float);
+        else if (type == GCN_BF16) NORM_LAUNCH_T(__bf16);
+        else NORM_LAUNCH_T(_Float16);
+#undef NORM_LAUNCH_T
+#undef NORM_LAUNCH
+        GCN_CHECK_LAUNCH("k_grad_norm");
+        done += blocks;
+    }
+    if (done > 0x7fffffffull) return fail(-2, "gcn_grad_norm: too many partial sums");
+    GCN_PROF_PRE("k_grad_norm_final");
+    k_grad_norm_final<<<1, 1024, 0, st>>>((int)done, part, grad_scale, max_norm, out);
+    GCN_CHECK_LAUNCH("k_grad_norm_final");
+    return 0;
+}
+
+}  // extern "C"

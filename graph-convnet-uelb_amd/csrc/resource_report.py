@@ -2,7 +2,7 @@
 """VGPR / AGPR / scratch / occupancy / LDS per kernel of the library (hipcc -Rpass-analysis=kernel-resource-usage)."""
 import os, re, subprocess, sys
 here = os.path.dirname(os.path.abspath(__file__))
-out = subprocess.run("/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -Xclang -target-feature -Xclang -packed-fp32-ops -Rpass-analysis=kernel-resource-usage -o /tmp/_gcn_rr.so api.hip",
+out = subprocess.run("/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -Xclang -target-feature -Xclang -packed-fp32-ops -Rpass-analysis=kernel-resource-usage -o /tmp/_gcn_rr.so *.hip",
                      shell=True, capture_output=True, text=True, cwd=here).stderr
 cur, rows = None, []
 for line in out.split('\n'):

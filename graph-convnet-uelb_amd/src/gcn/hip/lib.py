@@ -6,15 +6,16 @@ missing or a call fails, an exception is raised.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_size_t, c_void_p
 
 import torch
 
 _PKG_ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), "..", "..", ".."))
 LIB_PATH = os.environ.get("GCN_UELB_LIB") or os.path.join(_PKG_ROOT, "lib", "libgcn_uelb_hip.so")
-ABI_VERSION = 3
+ABI_VERSION = 4
 MAX_H = 320
 LAYER_NPARAMS = 12
 
@@ -26,7 +27,7 @@ class GcnHipError(RuntimeError):
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  Some forms of them have given wrong results now and then, and the edge
 # kernels lose nothing without them (headline step 0.656 -> 0.660 ms, 300 channels x 30 layers 96.4 -> 95.2 ms, same
 # losses).  The host pass warns that it does not know the feature: harmless.
-BUILD_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+BUILD_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
@@ -36,6 +37,16 @@ def source_files():
     files = sorted(os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".hip", ".hpp")))
     files.append(os.path.abspath(os.path.join(_PKG_ROOT, "..", "include", "gcn_uelb_hip.h")))
     return files
+
+
+def build_commands(hipcc, out):
+    """One compile command per translation unit (csrc/*.hip; they are independent of each other) and the link command."""
+    obj_dir = os.path.join(_PKG_ROOT, "build")
+    os.makedirs(obj_dir, exist_ok=True)
+    units = [f for f in source_files() if f.endswith(".hip")]
+    objs = [os.path.join(obj_dir, os.path.basename(f)[:-4] + ".o") for f in units]
+    return ([[hipcc, *BUILD_FLAGS, "-c", "-o", o, f] for f, o in zip(units, objs)],
+            [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out, *objs])
 
 
 def source_hash():
@@ -59,6 +70,15 @@ class ModelDesc(ctypes.Structure):
         ("mlp_layers", c_int), ("voc_out", c_int), ("n_emb", c_int), ("aggregation", c_int),
         ("training", c_int), ("mask_invalid_edges", c_int), ("has_labels", c_int),
         ("p_layer", c_float), ("p_mlp", c_float), ("advance_rng", c_int),
+    ]
+
+
+class AdamWDesc(ctypes.Structure):
+    """Mirror of ``gcn_adamw_desc`` (include/gcn_uelb_hip.h)."""
+    _fields_ = [
+        ("n", c_int), ("param_type", c_int), ("state_bits", c_int), ("first_tensor", ctypes.c_uint),
+        ("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+        ("step", ctypes.c_longlong), ("seed", ctypes.c_ulonglong),
     ]
 
 
@@ -151,6 +171,16 @@ def _declare(lib):
         lib.gcn_adam_step.restype = c_int
         lib.gcn_adam_step.argtypes = [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_float, ctypes.c_float,
                                       ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_longlong, c_void_p]
+    lib.gcn_adamw_hyper_bytes.restype = c_size_t
+    lib.gcn_adamw_hyper_bytes.argtypes = []
+    lib.gcn_adamw_advance.restype = c_int
+    lib.gcn_adamw_advance.argtypes = [POINTER(AdamWDesc)] + [c_void_p] * 4
+    lib.gcn_adamw_step.restype = c_int
+    lib.gcn_adamw_step.argtypes = [POINTER(AdamWDesc)] + [c_void_p] * 12
+    lib.gcn_grad_norm_ws_bytes.restype = c_size_t
+    lib.gcn_grad_norm_ws_bytes.argtypes = [c_int, c_void_p]
+    lib.gcn_grad_norm.restype = c_int
+    lib.gcn_grad_norm.argtypes = [c_int, c_int, c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_size_t, c_void_p]
 
 
 def load():
@@ -210,6 +240,13 @@ def ptr_array(tensors):
 
 def stream_ptr(device):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def device_guard(device):
+    """``torch.cuda.device(device)``, or nothing where that device is current already."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def require_cuda(t, name):

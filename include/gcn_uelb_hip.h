@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define GCN_ABI_VERSION 3
+#define GCN_ABI_VERSION 4
 #define GCN_MAX_H 320
 #define GCN_LAYER_NPARAMS 12
 #define GCN_MAX_MLP_LAYERS 4
@@ -295,6 +295,54 @@ int gcn_unpack_batch(int B, int V, int C, const unsigned char* edges_u8, const i
 int gcn_adam_step(int n, float* const* params, const float* const* grads, float* const* exp_avg,
                   float* const* exp_avg_sq, const long long* numel, float lr, float beta1, float beta2, float eps,
                   float weight_decay, long long step, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * AdamW update (decoupled weight decay) of n parameter tensors in one or a few launches, with the two moments in
+ * fp32 or in 8 bits.  The reference trains with torch.optim.Adam only (src/gcn/train/trainer.py:95).
+ *   g' = grad_scale * clip_coef * g ; m = b1 m + (1-b1) g' ; v = b2 v + (1-b2) g'^2 ;
+ *   p = (1 - lr wd) p - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * params / grads are of param_type.  16-bit parameters need `masters`: fp32 copies that take the update, the
+ * parameter becomes their rounding (and is not read); fp32 parameters take masters == NULL.
+ * state_bits 32: exp_avg / exp_avg_sq are fp32 [numel], the exponent arrays NULL.
+ * state_bits 8: exp_avg / exp_avg_sq are uint8 [numel], OCP e4m3 codes c in blocks of GCN_STATE8_BLOCK elements with one
+ *   exponent byte E per block ([ceil(numel / GCN_STATE8_BLOCK)]): m = e4m3(c) 2^(E-127), sqrt(v) = e4m3(c) 2^(E-127).
+ *   All zeros are the states of the first step.  The rounding to the codes is stochastic: a hash of (seed, step, number of the
+ *   tensor, element) gives the random bits, so equal calls give equal bits, also on different ranks.  The number of tensor k
+ *   is first_tensor + k.
+ * grad_scale, clip_coef: device scalars or NULL (= 1).  The gradients are not changed.  Tensors must not overlap.
+ * hyper: NULL, or device memory (gcn_adamw_hyper_bytes() bytes) that gcn_adamw_advance has filled: the step count, lr and
+ *   what depends on them are then read from there when the kernel runs, so that a captured graph can be replayed.
+ * gcn_adamw_advance adds 1 to *step (device memory) and fills hyper for that step; lr: device scalar, or NULL for desc.lr.
+ * ---------------------------------------------------------------------------------------------- */
+#define GCN_F32 0
+#define GCN_BF16 1
+#define GCN_F16 2
+#define GCN_STATE8_BLOCK 128
+
+typedef struct gcn_adamw_desc {
+    int n;                       /* tensors */
+    int param_type;              /* GCN_F32, GCN_BF16 or GCN_F16 */
+    int state_bits;              /* 32 or 8 */
+    unsigned int first_tensor;
+    double lr, beta1, beta2, eps, weight_decay;
+    long long step;              /* 1-based count of this update; ignored if hyper is given */
+    unsigned long long seed;
+} gcn_adamw_desc;
+
+size_t gcn_adamw_hyper_bytes(void);
+int gcn_adamw_advance(const gcn_adamw_desc* d, long long* step, const float* lr, void* hyper, void* stream);
+int gcn_adamw_step(const gcn_adamw_desc* d, void* const* params, const void* const* grads, float* const* masters,
+                   void* const* exp_avg, void* const* exp_avg_sq, unsigned char* const* exp_avg_exp,
+                   unsigned char* const* exp_avg_sq_exp, const long long* numel, const float* grad_scale,
+                   const float* clip_coef, const void* hyper, void* stream);
+
+/* Global norm of n gradient tensors of one type: out[0] = |grad_scale| * sqrt(sum of all squares), out[1] = min(1, max_norm /
+ * (out[0] + 1e-6)), the coefficient of torch.nn.utils.clip_grad_norm_ (the reference clips with it,
+ * src/gcn/training/reinforcement_strategy.py).  Squares are summed in double precision in a fixed order.  numel and
+ * the pointer arrays are host arrays, out is two floats in device memory, ws gcn_grad_norm_ws_bytes() bytes. */
+size_t gcn_grad_norm_ws_bytes(int n, const long long* numel);
+int gcn_grad_norm(int n, int type, const void* const* grads, const long long* numel, const float* grad_scale, double max_norm,
+                  float* out, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
