@@ -82,6 +82,16 @@ class AdamWDesc(ctypes.Structure):
     ]
 
 
+class LogitsDesc(ctypes.Structure):
+    """Mirror of ``gcn_logits_desc`` (include/gcn_uelb_hip.h)."""
+    _fields_ = ([(k, ctypes.c_longlong) for k in (
+        "rows", "vocab", "inner", "in_stride", "out_stride", "history_len", "history_rows", "bias_rows", "mask_rows",
+        "repetition_rows", "presence_rows", "frequency_rows", "temperature_rows")] + [(k, c_void_p) for k in (
+            "history", "history_lens", "prompt_lens", "mask", "bias", "repetition_t", "presence_t", "frequency_t", "temperature_t")]
+        + [(k, c_int) for k in ("type", "history_wide", "lens_wide", "mask_type")]
+        + [(k, c_float) for k in ("repetition", "presence", "frequency", "temperature", "masked_value")])
+
+
 _lib = None
 
 
@@ -181,6 +191,10 @@ def _declare(lib):
     lib.gcn_grad_norm_ws_bytes.argtypes = [c_int, c_void_p]
     lib.gcn_grad_norm.restype = c_int
     lib.gcn_grad_norm.argtypes = [c_int, c_int, c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.gcn_logits_process.restype = c_int
+    lib.gcn_logits_process.argtypes = [POINTER(LogitsDesc)] + [c_void_p] * 3
+    lib.gcn_logits_process_bwd.restype = c_int
+    lib.gcn_logits_process_bwd.argtypes = [POINTER(LogitsDesc)] + [c_void_p] * 5
 
 
 def load():

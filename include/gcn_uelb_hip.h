@@ -344,6 +344,45 @@ size_t gcn_grad_norm_ws_bytes(int n, const long long* numel);
 int gcn_grad_norm(int n, int type, const void* const* grads, const long long* numel, const float* grad_scale, double max_norm,
                   float* out, void* ws, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Rules on logits before something is drawn from them (penalties for tokens that occurred, bias, temperature, mask), and
+ * their gradient.  The reference masks scores inside the model and the sampler only (src/gcn/models/gcn_model.py:106-109,
+ * src/gcn/algorithms/path_sampler.py:86-114).
+ * in / out: [rows][vocab][inner] of `type`, rows in_stride / out_stride elements apart, dense within a row; out may be in.
+ * history: [history_rows][history_len] entries of the vocabulary (int32, or int64 if history_wide); entries outside
+ *   [0, vocab) are skipped; of row r the first history_lens[r] count (NULL: all).  For entry v of row o
+ *   n = its occurrences from place prompt_lens[r] on (NULL: from 0), seen = it occurs at any place:
+ *     x1 = seen ? (x > 0 ? x / repetition : x * repetition) : x
+ *     y  = (x1 - n * frequency - (n > 0) * presence + bias[v]) / temperature,   masked_value where the mask has v off
+ * Row o uses row o mod *_rows of each argument; *_rows divides rows.  repetition .. temperature: *_t (device, [*_rows])
+ * or, where that is NULL, the number; repetition and temperature are positive.
+ * mask_type 1: uint8 [mask_rows][vocab], 0 = off; 2: 32-bit words [mask_rows][ceil(vocab / 32)], lowest bit first, 0 = off.
+ * bias: float [bias_rows][vocab] or NULL.  A row whose mask leaves nothing becomes masked_value throughout.
+ * gcn_logits_process_bwd: dout and din have out_stride; din (NULL: not wanted) and dbias [bias_rows][vocab] (NULL likewise) are
+ *   overwritten; both are 0 where the mask has v off, whatever in and dout hold there.  At x = 0 the slope is that of
+ *   x < 0.  Sums are fp32 in a fixed order.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct gcn_logits_desc {
+    long long rows, vocab, inner;
+    long long in_stride, out_stride;
+    long long history_len, history_rows, bias_rows, mask_rows;
+    long long repetition_rows, presence_rows, frequency_rows, temperature_rows;
+    const void* history;
+    const void* history_lens;            /* int32, or int64 if lens_wide */
+    const void* prompt_lens;
+    const void* mask;
+    const float* bias;
+    const float* repetition_t;
+    const float* presence_t;
+    const float* frequency_t;
+    const float* temperature_t;
+    int type, history_wide, lens_wide, mask_type;
+    float repetition, presence, frequency, temperature, masked_value;
+} gcn_logits_desc;
+
+int gcn_logits_process(const gcn_logits_desc* d, const void* in, void* out, void* stream);
+int gcn_logits_process_bwd(const gcn_logits_desc* d, const void* in, const void* dout, void* din, float* dbias, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,326 @@
+"""Rules on logits and their gradient on the GPU against the formulas in double precision.
+
+Tolerances count roundings, u = 2^-24 each, and half a step (finfo.eps / 2) of the logits' type for the result:
+  y: |err| <= 8 u (|x1| + n |alpha_f| + |alpha_p| + |bias|) / tau + eps / 2 |y|       1/rho, product, penalty (2), sums (2), 1/tau, product
+  dx: |err| <= 4 u |dx| + eps / 2 |dx|
+  dbias: sums of N terms of 2 roundings each, in any order: |err| <= (N + 2) u sum |terms|
+fp16 adds its smallest subnormal step's half, 2^-25."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import logits_oracle as O
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a ROCm GPU")
+    return torch.device("cuda:0")
+
+
+def case(dev, rows, vocab, inner=1, length=20, dtype=torch.float32, seed=0, mask="bits", bias_rows=1, per_row=True, wide=True, hist_rows=None):
+    """Arguments of process_logits for logits [rows, vocab(, inner)], and those of the oracle."""
+    from src.gcn.hip.logits import pack_mask
+    rng = np.random.default_rng(seed)
+    hist_rows = rows if hist_rows is None else hist_rows
+    x = torch.from_numpy(3 * rng.standard_normal((rows, vocab, inner)).astype(np.float32)).to(dtype)
+    ints = torch.int64 if wide else torch.int32
+    few = rng.integers(-2, vocab + 2, max(1, length // 3) + 1)                   # entries that occur often, some of them invalid
+    hist = torch.from_numpy(np.where(rng.random((hist_rows, length)) < 0.5, rng.choice(few, (hist_rows, length)),
+                                     rng.integers(0, vocab, (hist_rows, length)))).to(ints)
+    lens = torch.from_numpy(rng.integers(-1, length + 2, hist_rows)).to(ints)
+    prompts = torch.from_numpy(rng.integers(0, length // 2 + 1, hist_rows)).to(ints)
+    number = lambda lo, hi: torch.from_numpy(rng.uniform(lo, hi, rows).astype(np.float32)) if per_row else round(float(rng.uniform(lo, hi)), 3)
+    rho, ap, af, tau = number(0.7, 1.6), number(-0.5, 1.0), number(-0.2, 0.5), number(0.4, 2.0)
+    bias = torch.from_numpy(rng.standard_normal((bias_rows, vocab)).astype(np.float32)) if bias_rows else None
+    allowed = None
+    if mask:
+        allowed = rng.random((rows, vocab)) < rng.random((rows, 1))
+        allowed[rows // 2] = False                                               # a row with nothing left
+        allowed = torch.from_numpy(allowed)
+    # rows shared by several leading positions: those of the last leading dimension
+    period = next((n for n in (bias_rows, hist_rows) if n not in (0, 1, rows)), None)
+    lead = (rows,) if period is None else (rows // period, period)
+    rows_of = lambda t: t.view(*(lead if t.shape[0] == rows and rows > 1 else t.shape[:1]), *t.shape[1:])
+    put = lambda t: rows_of(t).to(dev) if isinstance(t, torch.Tensor) else t
+    kind = dict(dim=len(lead), history=put(hist), history_lens=put(lens), prompt_lens=put(prompts), repetition_penalty=put(rho), presence_penalty=put(ap),
+                frequency_penalty=put(af), temperature=put(tau), bias=put(bias),
+                mask=None if allowed is None else put(pack_mask(allowed) if mask == "bits" else allowed))
+    np64 = lambda t: t.double().numpy() if isinstance(t, torch.Tensor) else t
+    want = dict(history=hist.numpy(), lens=lens.numpy(), prompts=prompts.numpy(), rho=np64(rho), alpha_p=np64(ap), alpha_f=np64(af), tau=np64(tau),
+                bias=None if bias is None else bias.numpy(), mask=None if allowed is None else allowed.numpy())
+    return x.to(dev).view((*lead, vocab) if inner == 1 else (*lead, vocab, inner)), kind, want
+
+
+def host(t, shape=None):
+    a = t.detach().double().cpu().numpy()
+    return a if shape is None else a.reshape(shape)
+
+
+def half_step(dtype):
+    return 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+
+
+def near(got, want, tol, masked=None):
+    finite = np.isfinite(want)
+    assert np.array_equal(finite, np.isfinite(got)) and np.array_equal(got[~finite], want[~finite], equal_nan=True)
+    off = np.abs(got[finite] - want[finite]) - tol[finite]
+    assert (off <= 0).all(), float(off.max())
+
+
+def check(x, kind, want, masked=-math.inf, out=None, got=None):
+    from src.gcn.hip.logits import process_logits
+    y = process_logits(x, masked_value=masked, out=out, **kind) if got is None else got
+    assert y.shape == x.shape and y.dtype == x.dtype
+    rows, vocab = math.prod(x.shape[:kind["dim"]]), x.shape[kind["dim"]]
+    ref, _, _, bound = O.process(host(x, (rows, vocab, -1)), masked=float(torch.tensor(masked, dtype=torch.float32).to(x.dtype)), **want)
+    near(host(y, ref.shape), ref, 8 * U * bound + half_step(x.dtype) * np.abs(np.nan_to_num(ref, neginf=0.0)) + 2.0 ** -25 * (x.dtype == torch.float16))
+    return y
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("vocab", [1, 7, 8, 31, 33, 2047, 2048, 2049, 5000])
+def test_rows_match_the_formula(dev, dtype, vocab):
+    for rows, length, mask, bias_rows, per_row, wide in ((1, 1, "bits", 1, True, True), (6, 40, "bits", 6, True, False), (6, 300, "bool", 3, False, True),
+                                                         (4, 17, None, 0, True, True)):
+        check(*case(dev, rows, vocab, length=length, dtype=dtype, seed=vocab, mask=mask, bias_rows=bias_rows, per_row=per_row, wide=wide))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("vocab, inner", [(1, 1), (1, 5), (14, 10), (33, 3), (200, 7), (9, 513), (2500, 2)])
+def test_inner_dimensions(dev, dtype, vocab, inner):
+    for mask, bias_rows, hist_rows in (("bool", 3, 3), ("bits", 6, 6), (None, 1, 1)):
+        check(*case(dev, 6, vocab, inner, length=25, dtype=dtype, seed=inner, mask=mask, bias_rows=bias_rows, per_row=False, hist_rows=hist_rows),
+              masked=-1e4)
+
+
+@pytest.mark.parametrize("rows, vocab, length", [(1, 100000, 3000), (3, 50021, 40000), (700, 3000, 64), (2, 131072, 1)])
+def test_long_rows_and_long_histories(dev, rows, vocab, length):
+    x, kind, want = case(dev, rows, vocab, length=length, dtype=torch.bfloat16, seed=3, mask="bits")
+    check(x, kind, want)
+
+
+def test_lengths_of_zero(dev):
+    from src.gcn.hip.logits import process_logits
+    x, kind, want = case(dev, 4, 100, length=9, seed=2)
+    empty = {**kind, "history": kind["history"][:, :0], "history_lens": None, "prompt_lens": None}
+    check(x, empty, {**want, "history": None})
+    none = {**kind, "history_lens": torch.zeros_like(kind["history_lens"])}
+    check(x, none, {**want, "lens": np.zeros(4)})
+    long_prompt = {**kind, "prompt_lens": torch.full_like(kind["prompt_lens"], 100)}
+    check(x, long_prompt, {**want, "prompts": np.full(4, 100)})
+    assert process_logits(x[:0], dim=1).shape == (0, 100)
+    assert torch.equal(process_logits(x), x)
+    with pytest.raises(ValueError, match="is on cpu"):
+        process_logits(x, history=kind["history"].cpu())
+
+
+def test_strided_rows_views_and_in_place(dev):
+    from src.gcn.hip.logits import process_logits
+    for dtype in TYPES:
+        x, kind, want = case(dev, 5, 1001, length=30, dtype=dtype, seed=5)
+        big = torch.full((5, 1100), 9.0, dtype=dtype, device=dev)
+        big[:, 3:1004] = x
+        view = big[:, 3:1004]
+        ref = check(view, kind, want)
+        assert torch.equal(ref, check(x, kind, want))
+        out = torch.full((5, 1003), 5.0, dtype=dtype, device=dev)
+        check(view, kind, want, out=out[:, 1:1002])
+        assert torch.equal(out[:, 1:1002], ref) and bool((out[:, 0] == 5).all()) and bool((out[:, 1002] == 5).all())
+        got = process_logits(view, out=view, masked_value=-math.inf, **kind)
+        assert got.data_ptr() == view.data_ptr() and torch.equal(view, ref)
+        assert bool((big[:, :3] == 9).all()) and bool((big[:, 1004:] == 9).all())
+        steps = x.repeat_interleave(2, 1)[:, ::2]                     # every second element
+        assert torch.equal(process_logits(steps, **kind), ref)
+        cols = x.t().contiguous().t()
+        assert torch.equal(process_logits(cols, **kind), ref)
+        same = x[:1].expand(5, -1)
+        check(same, kind, want)
+        three = torch.stack([x, x]).transpose(0, 1)                   # [5, 2, V], the rows not evenly spaced
+        lead = {**{k: v for k, v in kind.items() if k in ("temperature", "bias")}, "dim": 2}
+        lead["temperature"] = kind["temperature"].view(5, 1).expand(5, 2)
+        assert torch.equal(process_logits(three, **lead)[:, 0], process_logits(x, dim=1, temperature=kind["temperature"], bias=kind["bias"]))
+
+
+def test_leading_dimensions_and_shared_rows(dev):
+    """[B, V, V, C] scores: history, bias and mask of all graphs, of every graph, of one node; all equal their expanded forms."""
+    from src.gcn.hip.logits import process_logits
+    gen = torch.Generator(dev).manual_seed(0)
+    y = torch.randn(3, 5, 7, 2, device=dev, generator=gen)
+    hist = torch.randint(-1, 7, (5, 4), device=dev, generator=gen)
+    bias, mask = torch.randn(5, 7, device=dev, generator=gen), torch.rand(5, 7, device=dev, generator=gen) < 0.6
+    got = process_logits(y, dim=2, history=hist, bias=bias, mask=mask, repetition_penalty=1.5, frequency_penalty=0.3, masked_value=-1e9)
+    want = process_logits(y.reshape(15, 7, 2), dim=1, history=hist.repeat(3, 1), bias=bias.repeat(3, 1), mask=mask.repeat(3, 1), repetition_penalty=1.5,
+                          frequency_penalty=0.3, masked_value=-1e9).view(y.shape)
+    assert torch.equal(got, want)
+    one = process_logits(y, dim=-2, history=hist[:1], bias=bias[0], mask=mask[:1], masked_value=-1e9)
+    two = process_logits(y, dim=2, history=hist[:1].expand(3, 5, 4), bias=bias[0].expand(3, 5, 7), mask=mask[0].expand(3, 5, 7), masked_value=-1e9)
+    assert torch.equal(one, two)
+
+
+def test_bad_values_in_masked_places_and_outside(dev):
+    from src.gcn.hip.logits import process_logits
+    x = torch.tensor([[float("nan"), float("inf"), -float("inf"), 1.0, -2.0, float("nan"), -float("inf"), 3.0]], device=dev)
+    on = torch.tensor([[0, 0, 0, 1, 1, 1, 1, 1]], device=dev, dtype=torch.bool)
+    hist = torch.tensor([[0, 3, 4, 4, 6]], device=dev)
+    for dtype in TYPES:
+        for masked in (-math.inf, float(torch.finfo(dtype).min), 0.0):
+            y = process_logits(x.to(dtype), history=hist, repetition_penalty=2.0, frequency_penalty=0.5, mask=on, masked_value=masked)
+            want = [masked] * 3 + [0.0, -5.0, float("nan"), -math.inf, 3.0]
+            assert np.array_equal(host(y)[0], np.array(want), equal_nan=True)
+    z = x.clone().requires_grad_()
+    bias = torch.zeros(8, device=dev, requires_grad=True)
+    y = process_logits(z, history=hist, repetition_penalty=2.0, bias=bias, mask=on)
+    dy = torch.tensor([[float("nan"), float("inf"), 1.0, 1.0, 1.0, 1.0, 1.0, 1.0]], device=dev)
+    dx, db = torch.autograd.grad(y, [z, bias], dy)
+    assert host(dx)[0].tolist() == [0, 0, 0, 0.5, 2, 1, 2, 1] and host(db).tolist() == [0, 0, 0, 1, 1, 1, 1, 1]
+
+
+def grads(x, kind, want, bias_rows, dy, masked=-1e4):
+    from src.gcn.hip.logits import process_logits
+    z, b = x.detach().requires_grad_(), None if kind["bias"] is None else kind["bias"].clone().requires_grad_()
+    y = process_logits(z, masked_value=masked, **{**kind, "bias": b})
+    check(x, kind, want, masked=masked, got=y)
+    got = torch.autograd.grad(y, [z] if b is None else [z, b], dy)
+    rows, vocab = math.prod(x.shape[:kind["dim"]]), x.shape[kind["dim"]]
+    shape = (rows, vocab, x.numel() // (rows * vocab))
+    _, slope, slope_b, _ = O.process(host(x, shape), masked=masked, **want)
+    dx, db, size = O.gradient(host(dy, shape), slope, slope_b, max(bias_rows, 1))
+    eps = half_step(x.dtype)
+    assert got[0].dtype == x.dtype and got[0].shape == x.shape
+    assert (np.abs(host(got[0], shape) - dx) <= (4 * U + eps) * np.abs(dx) + 2.0 ** -25 * (x.dtype == torch.float16)).all()
+    if b is not None:
+        terms = shape[2] * rows // bias_rows
+        assert got[1].dtype == torch.float32 and got[1].shape == kind["bias"].shape
+        assert (np.abs(host(got[1]) - db) <= (terms + 2) * U * size + 1e-44).all()
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows, vocab, inner, bias_rows", [
+    (1, 1, 1, 1), (6, 2049, 1, 1), (6, 33, 1, 3), (6, 100, 1, 6), (6, 100, 1, 0), (12, 14, 10, 4), (12, 14, 10, 12), (12, 14, 10, 1), (8, 200, 100, 4),
+    (3, 5, 700, 3), (2, 9, 4097, 1), (300, 50, 1, 1), (513, 2500, 1, 1), (64, 17, 3, 2)])
+def test_gradient_matches_the_formula(dev, dtype, rows, vocab, inner, bias_rows):
+    for mask, per_row in (("bits", True), ("bool", False), (None, False)):
+        x, kind, want = case(dev, rows, vocab, inner, length=20, dtype=dtype, seed=rows, mask=mask, bias_rows=bias_rows, per_row=per_row)
+        dy = torch.randn(x.shape, device=dev, generator=torch.Generator(dev).manual_seed(1)).to(dtype)
+        first = grads(x, kind, want, bias_rows, dy)
+        again = grads(x, kind, want, bias_rows, dy)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))                  # the same bits every time
+
+
+def test_gradient_with_strides_and_broadcasts(dev):
+    from src.gcn.hip.logits import process_logits
+    x, kind, want = case(dev, 6, 40, 3, seed=4, bias_rows=2, per_row=False)          # logits [3, 2, 40, 3]
+    dy = torch.randn(3, 2, 40, 3, device=dev)
+    base = grads(x, kind, want, 2, dy)
+    part = torch.zeros(3, 2, 50, 3, device=dev)
+    part[:, :, 2:42] = x
+    assert all(torch.equal(a, b) for a, b in zip(base, grads(part[:, :, 2:42], kind, want, 2, dy)))
+    assert all(torch.equal(a, b) for a, b in zip(base, grads(x, kind, want, 2, dy.permute(3, 1, 0, 2).contiguous().permute(2, 1, 3, 0))))
+    one = torch.ones((), device=dev).expand(3, 2, 40, 3)                             # what sum().backward() passes
+    grads(x, kind, want, 2, one)
+    # an expanded bias and expanded logits: autograd adds over the expansion
+    b = torch.randn(40, device=dev, requires_grad=True)
+    z = x[:1, :1].clone().requires_grad_()
+    y = process_logits(z.expand(3, 2, 40, 3), **{**kind, "bias": b.expand(2, 40)}, masked_value=0.0)
+    dz, db = torch.autograd.grad(y, [z, b], dy)
+    z2, b2 = x[:1, :1].repeat(3, 2, 1, 1).requires_grad_(), b.detach().requires_grad_()
+    y2 = process_logits(z2, **{**kind, "bias": b2}, masked_value=0.0)
+    dz2, db2 = torch.autograd.grad(y2, [z2, b2], dy)
+    # sums of at most 18 terms, in two orders
+    assert float((dz - dz2.sum((0, 1), keepdim=True)).abs().max()) <= 2 * 18 * U * float(dz2.abs().sum((0, 1)).max())
+    assert float((db - db2).abs().max()) <= 2 * 18 * U * 18 * float(dz2.abs().max() + dy.abs().max())
+    # only one of the two
+    y = process_logits(x, **{**kind, "bias": b2}, masked_value=0.0)
+    (only,) = torch.autograd.grad(y, [b2], dy)
+    z = x.detach().requires_grad_()
+    _, both = torch.autograd.grad(process_logits(z, **{**kind, "bias": b2}, masked_value=0.0), [z, b2], dy)
+    assert torch.equal(only, both)
+    (only,) = torch.autograd.grad(process_logits(z, **kind, masked_value=0.0), [z], dy)
+    assert torch.equal(only, torch.autograd.grad(process_logits(z, **{**kind, "bias": None}, masked_value=0.0), [z], dy)[0])
+
+
+def test_changed_inputs_are_noticed_by_backward(dev):
+    from src.gcn.hip.logits import process_logits
+    x, kind, _ = case(dev, 3, 20, seed=1)
+    z = x.detach().requires_grad_()
+    y = process_logits(z, **kind)
+    kind["history"].zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = process_logits(z, **kind)
+    with pytest.raises(RuntimeError, match="once_differentiable|differentiat"):
+        (g,) = torch.autograd.grad(y.masked_fill(y.isinf(), 0).square().sum(), [z], create_graph=True)
+        g.sum().backward()
+
+
+def test_capture_forward_and_backward(dev):
+    """Replays on new inputs, with eager work between them, against eager calls."""
+    from src.gcn.hip.logits import process_logits
+    x, kind, _ = case(dev, 16, 3000, length=50, dtype=torch.bfloat16, seed=6)
+    dy = torch.randn(x.shape, device=dev).to(x.dtype)
+    bias = kind.pop("bias")
+
+    def both():
+        z, b = x.detach().requires_grad_(), bias.detach().requires_grad_()
+        y = process_logits(z, bias=b, masked_value=-1e4, **kind)
+        return [y.detach(), *torch.autograd.grad(y, [z, b], dy)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = both()
+    with torch.cuda.graph(second):
+        other = both()
+    for k in range(4):
+        x.copy_(torch.randn(x.shape, device=dev))
+        kind["history"].copy_(torch.randint(0, 3000, kind["history"].shape, device=dev))
+        graph.replay()
+        second.replay()
+        torch.cuda.synchronize()
+        want = both()
+        for a, b, c in zip(static, want, other):
+            assert torch.equal(a, b) and torch.equal(a, c), k
+
+
+def test_two_streams(dev):
+    from src.gcn.hip.logits import process_logits
+    jobs = [case(dev, 40, 20000, length=200, seed=s, bias_rows=1) for s in (1, 2)]
+    want = [process_logits(x, **kind) for x, kind, _ in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for st, (x, kind, _) in zip(streams, jobs):
+        with torch.cuda.stream(st):
+            got.append(process_logits(x, **kind))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_offsets_beyond_32_bits(dev):
+    """More than 2^31 elements: the last rows against the same rows alone."""
+    from src.gcn.hip.logits import process_logits
+    rows, vocab = 17000, 131072
+    x = torch.empty(rows, vocab, dtype=torch.bfloat16, device=dev).normal_(generator=torch.Generator(dev).manual_seed(0))
+    hist = torch.randint(0, vocab, (rows, 8), device=dev)
+    bias = torch.randn(vocab, device=dev)
+    kind = dict(repetition_penalty=1.3, frequency_penalty=0.5, bias=bias)
+    y = process_logits(x, history=hist, **kind)
+    for part in (slice(0, 3), slice(16380, 16390), slice(rows - 3, rows)):
+        assert torch.equal(y[part], process_logits(x[part], history=hist[part], **kind))
+    z = x.requires_grad_()
+    y = process_logits(z, history=hist, **kind)
+    (dx,) = torch.autograd.grad(y, [z], y.detach())
+    last = x[-3:].detach().requires_grad_()
+    (ref,) = torch.autograd.grad(process_logits(last, history=hist[-3:], **kind), [last], y[-3:].detach())
+    assert torch.equal(dx[-3:], ref)

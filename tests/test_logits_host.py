@@ -1,0 +1,117 @@
+"""Rules on logits: refusals and host-side checks; no GPU needed."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import logits_oracle as O
+from src.gcn.hip import lib as L
+from src.gcn.hip.logits import _row_stride, pack_mask, process_logits
+
+X = torch.zeros(2, 3, 10)
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(L.GcnHipError, match="no CPU fallback"):
+        process_logits(X)
+
+
+@pytest.mark.parametrize("kind, error", [
+    (dict(dim=3), ValueError),
+    (dict(history=torch.zeros(2, 3, 4)), TypeError),
+    (dict(history=torch.zeros(2, 4, dtype=torch.int64)), ValueError),
+    (dict(history=torch.zeros(3, 2, 4, dtype=torch.int64)), ValueError),
+    (dict(history=torch.zeros(2, 2, 3, 4, dtype=torch.int64)), ValueError),
+    (dict(history_lens=torch.zeros(3, dtype=torch.int64)), ValueError),
+    (dict(history=torch.zeros(3, 4, dtype=torch.int64), history_lens=torch.zeros(2, dtype=torch.int64)), ValueError),
+    (dict(history=torch.zeros(3, 4, dtype=torch.int64), history_lens=torch.zeros(3)), TypeError),
+    (dict(history=torch.zeros(3, 4, dtype=torch.int64), history_lens=torch.zeros(3, dtype=torch.int64),
+          prompt_lens=torch.zeros(3, dtype=torch.int32)), TypeError),
+    (dict(repetition_penalty=0.0), ValueError), (dict(repetition_penalty=float("nan")), ValueError), (dict(temperature=0.0), ValueError),
+    (dict(temperature=-1.0), ValueError), (dict(presence_penalty=float("inf")), ValueError),
+    (dict(temperature=torch.ones(3, dtype=torch.float64)), TypeError), (dict(temperature=torch.ones(2)), ValueError),
+    (dict(mask=torch.ones(3, 10)), TypeError), (dict(mask=torch.ones(3, 9, dtype=torch.bool)), ValueError),
+    (dict(mask=torch.ones(3, 2, dtype=torch.int32)), ValueError), (dict(mask=torch.ones(2, 10, dtype=torch.bool)), ValueError),
+    (dict(bias=torch.ones(10, dtype=torch.bfloat16)), TypeError), (dict(bias=torch.ones(11)), ValueError),
+    (dict(bias=torch.ones(2, 10)), ValueError), (dict(out=torch.zeros(2, 3, 9)), ValueError),
+    (dict(out=torch.zeros(2, 3, 20)[:, :, ::2]), ValueError), (dict(out=torch.zeros(10).expand(2, 3, 10)), ValueError),
+    (dict(out=torch.zeros(2, 3, 10, dtype=torch.float16)), ValueError),
+])
+def test_bad_arguments_are_refused(kind, error):
+    with pytest.raises(error):
+        process_logits(X, **kind)
+
+
+def test_other_refusals():
+    with pytest.raises(TypeError):
+        process_logits(X.double())
+    with pytest.raises(ValueError):
+        process_logits(torch.zeros(()))
+    with pytest.raises(ValueError, match="gradients"):
+        process_logits(X.clone().requires_grad_(), out=torch.zeros(2, 3, 10))
+
+
+def test_pack_mask():
+    gen = torch.Generator().manual_seed(0)
+    for v in (1, 31, 32, 33, 100):
+        m = torch.rand(3, v, generator=gen) < 0.5
+        w = pack_mask(m)
+        assert w.shape == (3, -(-v // 32)) and w.dtype == torch.int32
+        bits = np.unpackbits(w.numpy().view(np.uint8), axis=1, bitorder="little")[:, :v]
+        assert np.array_equal(bits.astype(bool), m.numpy())
+    with pytest.raises(TypeError):
+        pack_mask(torch.ones(3))
+
+
+def test_row_stride():
+    x = torch.zeros(4, 6, 10)
+    assert _row_stride(x, 2) == 10 and _row_stride(x, 1) == 60 and _row_stride(x, 0) == 240
+    assert _row_stride(x[:, :, :7], 2) == 10 and _row_stride(x[:, :, ::2], 2) is None
+    assert _row_stride(x[:, :3], 2) is None                       # rows not evenly spaced
+    assert _row_stride(x[:1, :3], 2) == 10 and _row_stride(x[:, :1], 2) == 60
+    assert _row_stride(torch.zeros(10).expand(4, 10), 1) == 0
+    assert _row_stride(x.transpose(0, 1), 2) is None
+
+
+def test_c_entry_points_refuse_without_touching_memory():
+    lib = L.load()
+    ok = dict(rows=4, vocab=8, inner=1, in_stride=8, out_stride=8, history_rows=1, bias_rows=1, mask_rows=1, repetition_rows=1, presence_rows=1,
+              frequency_rows=1, temperature_rows=1, type=0, repetition=1.0, temperature=1.0)
+
+    def call(**k):
+        d = L.LogitsDesc(**{**ok, **k})
+        return lib.gcn_logits_process(ctypes.byref(d), None, None, None)
+
+    assert call() == -1 and b"null pointer" in lib.gcn_last_error()
+    assert lib.gcn_logits_process(None, None, None, None) == -1
+    assert call(rows=0) == 0
+    for bad in (dict(type=3), dict(vocab=0), dict(inner=0), dict(rows=-1), dict(out_stride=7), dict(in_stride=-1), dict(mask_type=1),
+                dict(mask_type=3, mask=16), dict(mask=16), dict(repetition=0.0), dict(temperature=float("nan")), dict(history_lens=16),
+                dict(history=16, history_len=-1), dict(history=16, history_len=5, history_rows=3), dict(bias=16, bias_rows=3),
+                dict(mask=16, mask_type=2, mask_rows=5), dict(temperature_t=16, temperature_rows=0)):
+        assert call(**bad) == -1, bad
+        assert b"null pointer" not in lib.gcn_last_error(), bad
+    for big in (dict(vocab=1 << 31, out_stride=1 << 31), dict(vocab=1 << 20, inner=1 << 11, out_stride=1 << 31), dict(rows=1 << 31)):
+        assert call(**big) == -2, big
+    d = L.LogitsDesc(**ok)
+    assert lib.gcn_logits_process_bwd(ctypes.byref(d), None, None, None, 16, None) == -1 and b"bias" in lib.gcn_last_error()
+    assert lib.gcn_logits_process_bwd(ctypes.byref(d), 16, 16, None, None, None) == -1
+
+
+def test_oracle_gradient_against_differences():
+    rng = np.random.default_rng(1)
+    x, b = rng.standard_normal((4, 6, 3)), rng.standard_normal((2, 6))
+    hist = rng.integers(-1, 7, (2, 5))
+    mask = rng.random((4, 6)) < 0.7
+    kind = dict(history=hist, prompts=[1, 0], rho=1.3, alpha_p=0.2, alpha_f=0.1, mask=mask, tau=np.array([0.5, 2.0]), masked=-3.0)
+    dy = rng.standard_normal(x.shape)
+    _, slope, slope_b, _ = O.process(x, bias=b, **kind)
+    dx, db, _ = O.gradient(dy, slope, slope_b, 2)
+    f = lambda x, b: float((O.process(x, bias=b, **kind)[0] * dy).sum())
+    for grad, arr, at in ((dx, x, 0), (db, b, 1)):
+        for k in np.ndindex(arr.shape):
+            step = np.zeros_like(arr)
+            step[k] = 1e-6
+            args = [(x + step, b), (x - step, b)] if at == 0 else [(x, b + step), (x, b - step)]
+            assert abs((f(*args[0]) - f(*args[1])) / 2e-6 - grad[k]) < 1e-6
