@@ -11,13 +11,15 @@
 // Everything is fp32 and rounded once to the logits' type.
 //
 // Bound by memory: one read and one write of the logits (backward: of the gradient; a logit is read where its token is seen).
-// A workgroup takes a range of one row's vocabulary and counts the row's history into LDS first (integer atomics: the order
-// does not matter), so that there is one launch, no workspace and no second pass over the logits.
+// A workgroup takes a range of one row's vocabulary and counts the row's history into LDS (integer atomics: the order does not
+// matter) while its logits are on the way, so that there is one launch, no workspace and no second pass over the logits.
+// The backward pass takes a range of the rows that share a bias row, one after the other, and keeps the bias gradient's sums
+// in registers: the gradient is read once for both results.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#define LGT_THREADS 256
+#define LGT_THREADS 512                        // four workgroups on a CU: 32 wavefronts
 #define LGT_PER_LANE 8                         // consecutive elements of a lane
 #define LGT_STRIDE (LGT_THREADS * LGT_PER_LANE)
 #define LGT_SEEN 0x80000000u                   // a count's flag: the token stands in the prompt
@@ -37,6 +39,8 @@ struct LogitsArgs {
     const void* mask;
     const float *bias, *rep, *pres, *freq, *temp;      // rep .. temp: null = the number below
     float rep_value, pres_value, freq_value, temp_value, masked_value;
+    int splits;                    // backward: parts of the rows that share a bias row
+    float* dbias;                  // backward: [splits][bias_rows][vocab] or null
 };
 
 __device__ __forceinline__ float lgt_param(const float* p, int rows, float value, int o) { return p ? p[rows == 1 ? 0 : o % rows] : value; }
@@ -44,22 +48,44 @@ __device__ __forceinline__ long long lgt_int(const void* p, int wide, long long 
     return wide ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
 }
 
-// Counts of the entries [v0, v0 + n) in row o's history, into LDS.
+template <typename T, int N>
+struct LgtVecOf {
+    typedef T type __attribute__((ext_vector_type(N)));
+    typedef type loose __attribute__((aligned(sizeof(T))));      // rows of odd lengths: aligned to elements only
+};
+template <typename T, int N>
+using LgtVec = typename LgtVecOf<T, N>::type;
+template <typename T, int N>
+__device__ __forceinline__ LgtVec<T, N> lgt_vec(const T* p) { return *reinterpret_cast<const typename LgtVecOf<T, N>::loose*>(p); }
+
+// Counts of the entries [v0, v0 + n) in row o's history, into LDS.  Between two barriers of the workgroup.
+__device__ __forceinline__ void lgt_count_one(long long id, long long l, long long prompt, int v0, int n, uint32_t* cnt) {
+    const unsigned long long at = (unsigned long long)(id - v0);
+    if (at < (unsigned long long)n) {
+        if (l >= prompt) atomicAdd(&cnt[at], 1u);
+        else atomicOr(&cnt[at], LGT_SEEN);
+    }
+}
+template <typename ID>
+__device__ __forceinline__ void lgt_count_ids(const ID* __restrict__ ids, long long len, long long prompt, int v0, int n, uint32_t* cnt) {
+    constexpr int W = 16 / sizeof(ID);
+    long long l = (long long)threadIdx.x * W;
+    for (; l + W <= len; l += LGT_THREADS * W) {
+        const LgtVec<ID, W> some = lgt_vec<ID, W>(ids + l);
+#pragma unroll
+        for (int k = 0; k < W; ++k) lgt_count_one(some[k], l + k, prompt, v0, n, cnt);
+    }
+    for (; l < len; ++l) lgt_count_one(ids[l], l, prompt, v0, n, cnt);       // the one lane whose group is cut off
+}
 __device__ __forceinline__ void lgt_count(const LogitsArgs& a, int o, int v0, int n, uint32_t* cnt) {
-    for (int k = threadIdx.x; k < n; k += LGT_THREADS) cnt[k] = 0;
+    for (int k = threadIdx.x * 4; k < n; k += LGT_THREADS * 4) *reinterpret_cast<uint4*>(cnt + k) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     const int r = o % a.history_rows;
     long long len = a.lens ? lgt_int(a.lens, a.lens_wide, r) : a.history_len;
     len = len < a.history_len ? len : a.history_len;
-    const long long prompt = a.prompts ? lgt_int(a.prompts, a.lens_wide, r) : 0;
-    const long long base = (long long)r * a.history_len;
-    for (long long l = threadIdx.x; l < len; l += LGT_THREADS) {
-        const long long id = lgt_int(a.history, a.history_wide, base + l) - v0;
-        if (id >= 0 && id < n) {
-            if (l >= prompt) atomicAdd(&cnt[id], 1u);
-            else atomicOr(&cnt[id], LGT_SEEN);
-        }
-    }
+    const long long prompt = a.prompts ? lgt_int(a.prompts, a.lens_wide, r) : 0, base = (long long)r * a.history_len;
+    if (a.history_wide) lgt_count_ids(static_cast<const long long*>(a.history) + base, len, prompt, v0, n, cnt);
+    else lgt_count_ids(static_cast<const int*>(a.history) + base, len, prompt, v0, n, cnt);
     __syncthreads();
 }
 
@@ -70,86 +96,308 @@ __device__ __forceinline__ bool lgt_on(const LogitsArgs& a, int r, int v) {
     const int words = (a.vocab + 31) >> 5;
     return (static_cast<const uint32_t*>(a.mask)[(long long)r * words + (v >> 5)] >> (v & 31)) & 1;
 }
+// The same for eight entries from v on, a multiple of 8, of which `left` exist: bit k for v + k.
+__device__ __forceinline__ uint32_t lgt_on8(const LogitsArgs& a, int r, int v, int left) {
+    if (a.mask_type == 0) return 0xFFu;
+    if (left <= 0) return 0;
+    if (a.mask_type == 2) return static_cast<const uint8_t*>(a.mask)[(long long)r * (((a.vocab + 31) >> 5) * 4) + (v >> 3)];
+    const uint8_t* m = static_cast<const uint8_t*>(a.mask) + (long long)r * a.vocab + v;
+    uint32_t on = 0;
+    if (left >= LGT_PER_LANE) {
+        const LgtVec<uint8_t, LGT_PER_LANE> some = lgt_vec<uint8_t, LGT_PER_LANE>(m);
+#pragma unroll
+        for (int k = 0; k < LGT_PER_LANE; ++k) on |= (some[k] != 0 ? 1u : 0u) << k;
+    } else {
+        for (int k = 0; k < left; ++k) on |= (m[k] != 0 ? 1u : 0u) << k;
+    }
+    return on;
+}
 
-template <typename T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) LgtVec {      // rows of odd lengths: aligned to elements only
-    T v[N];
-};
+template <typename T>
+__device__ __forceinline__ LgtVec<T, LGT_PER_LANE> lgt_load(const T* p, long long e, int left) {
+    LgtVec<T, LGT_PER_LANE> raw;
+    if (left >= LGT_PER_LANE) {
+        raw = lgt_vec<T, LGT_PER_LANE>(p + e);
+    } else {
+#pragma unroll
+        for (int k = 0; k < LGT_PER_LANE; ++k) raw[k] = k < left ? p[e + k] : (T)0.f;
+    }
+    return raw;
+}
+template <typename T>
+__device__ __forceinline__ void lgt_store(T* p, long long e, int left, const float* out) {
+    if (left >= LGT_PER_LANE) {
+        LgtVec<T, LGT_PER_LANE> raw;
+#pragma unroll
+        for (int k = 0; k < LGT_PER_LANE; ++k) raw[k] = (T)out[k];
+        *reinterpret_cast<typename LgtVecOf<T, LGT_PER_LANE>::loose*>(p + e) = raw;
+    } else {
+#pragma unroll
+        for (int k = 0; k < LGT_PER_LANE; ++k)
+            if (k < left) p[e + k] = (T)out[k];
+    }
+}
 
-template <typename T, bool BACKWARD>
+// ---------------------------------------------------------------------------------------------- token logits (inner = 1)
+template <typename T, int ITER>
 __global__ __launch_bounds__(LGT_THREADS) void k_logits(LogitsArgs a) {
-    extern __shared__ uint32_t cnt[];
-    const int o = blockIdx.x / a.chunks, v0 = (blockIdx.x % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0);
-    if (a.history) lgt_count(a, o, v0, n, cnt);
+    extern __shared__ __align__(16) uint32_t cnt[];
+    const int o = blockIdx.x / a.chunks, v0 = (blockIdx.x % a.chunks) * (ITER * LGT_STRIDE), n = min(ITER * LGT_STRIDE, a.vocab - v0);
+    const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + v0;
+    T* y = static_cast<T*>(a.y) + (long long)o * a.y_stride + v0;
+    const int mask_row = a.mask_type ? o % a.mask_rows : 0;
+    const float* bias = a.bias ? a.bias + (long long)(o % a.bias_rows) * a.vocab + v0 : nullptr;
+    LgtVec<T, LGT_PER_LANE> raw[ITER];
+    uint32_t on[ITER];
+#pragma unroll
+    for (int t = 0; t < ITER; ++t) {
+        const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE;
+        raw[t] = lgt_load(x, e, n - e);
+        on[t] = lgt_on8(a, mask_row, v0 + e, n - e);
+    }
     const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
     const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
     const float pres = lgt_param(a.pres, a.pres_rows, a.pres_value, o), freq = lgt_param(a.freq, a.freq_rows, a.freq_value, o);
-    const float* bias = a.bias && !BACKWARD ? a.bias + (long long)(o % a.bias_rows) * a.vocab : nullptr;
-    const int mask_row = a.mask_type ? o % a.mask_rows : 0;
-    const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride;
-    const T* dy = BACKWARD ? static_cast<const T*>(a.dy) + (long long)o * a.y_stride : nullptr;
-    T* y = static_cast<T*>(a.y) + (long long)o * a.y_stride;
-    const int first = v0 * a.inner, end = first + n * a.inner;
-    for (int e = first + threadIdx.x * LGT_PER_LANE; e < end; e += LGT_STRIDE) {
-        const int left = min(end - e, LGT_PER_LANE);
-        float in[LGT_PER_LANE];
-        const T* src = BACKWARD ? dy : x;
-        if (left == LGT_PER_LANE) {
-            const LgtVec<T, LGT_PER_LANE> raw = *reinterpret_cast<const LgtVec<T, LGT_PER_LANE>*>(src + e);
+    if (a.history) lgt_count(a, o, v0, n, cnt);
 #pragma unroll
-            for (int k = 0; k < LGT_PER_LANE; ++k) in[k] = (float)raw.v[k];
-        } else {
-            for (int k = 0; k < LGT_PER_LANE; ++k) in[k] = k < left ? (float)src[e + k] : 0.f;
-        }
-        float out[LGT_PER_LANE];
-        int v = e / a.inner, i = e - v * a.inner;
+    for (int t = 0; t < ITER; ++t) {
+        const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE, left = n - e;
+        if (left <= 0) break;
+        float z[LGT_PER_LANE];
 #pragma unroll
-        for (int k = 0; k < LGT_PER_LANE; ++k) {
-            out[k] = 0.f;
-            if (k < left) {
-                const uint32_t c = a.history ? cnt[v - v0] : 0;
-                const bool on = lgt_on(a, mask_row, v);
-                float z = in[k];
-                if (BACKWARD) {
-                    z *= inv_tau;
-                    if (c) z *= (float)x[e + k] > 0.f ? inv_rho : rho;
-                    out[k] = on ? z : 0.f;
-                } else {
-                    const uint32_t times = c & ~LGT_SEEN;
-                    if (c) z *= z > 0.f ? inv_rho : rho;
-                    if (times) z -= (float)times * freq + pres;
-                    if (bias) z += bias[v];
-                    out[k] = on ? z * inv_tau : a.masked_value;
+        for (int k = 0; k < LGT_PER_LANE; ++k) z[k] = (float)raw[t][k];
+        if (a.history) {
+            uint32_t c[LGT_PER_LANE];
+            *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(cnt + e);
+            *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(cnt + e + 4);
+            if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
+#pragma unroll
+                for (int k = 0; k < LGT_PER_LANE; ++k) {
+                    const uint32_t times = c[k] & ~LGT_SEEN;
+                    if (c[k]) z[k] *= z[k] > 0.f ? inv_rho : rho;
+                    if (times) z[k] -= (float)times * freq + pres;
                 }
-                if (++i == a.inner) { i = 0; ++v; }
             }
         }
-        if (left == LGT_PER_LANE) {
-            LgtVec<T, LGT_PER_LANE> raw;
+        if (bias) {
+            const LgtVec<float, LGT_PER_LANE> b = lgt_load(bias, e, left);
 #pragma unroll
-            for (int k = 0; k < LGT_PER_LANE; ++k) raw.v[k] = (T)out[k];
-            *reinterpret_cast<LgtVec<T, LGT_PER_LANE>*>(y + e) = raw;
-        } else {
-            for (int k = 0; k < left; ++k) y[e + k] = (T)out[k];
+            for (int k = 0; k < LGT_PER_LANE; ++k) z[k] += b[k];
+        }
+#pragma unroll
+        for (int k = 0; k < LGT_PER_LANE; ++k) z[k] = (on[t] >> k) & 1 ? z[k] * inv_tau : a.masked_value;
+        lgt_store(y, e, left, z);
+    }
+}
+
+// Rows r, r + R, ... (R = bias_rows) of one part, one after the other: the gradient of the logits row by row, that of the bias
+// in registers.
+template <typename T, int ITER>
+__global__ __launch_bounds__(LGT_THREADS) void k_logits_bwd(LogitsArgs a) {
+    extern __shared__ __align__(16) uint32_t cnt[];
+    uint32_t at = blockIdx.x;
+    const int v0 = (int)(at % a.chunks) * (ITER * LGT_STRIDE), n = min(ITER * LGT_STRIDE, a.vocab - v0);
+    at /= a.chunks;
+    const int r = (int)(at % a.bias_rows), part = (int)(at / a.bias_rows), many = a.rows / a.bias_rows;
+    const int first = (int)((long long)many * part / a.splits), last = (int)((long long)many * (part + 1) / a.splits);
+    float sum[ITER][LGT_PER_LANE] = {};
+    for (int q = first; q < last; ++q) {
+        const int o = r + q * a.bias_rows, mask_row = a.mask_type ? o % a.mask_rows : 0;
+        const T* dy = static_cast<const T*>(a.dy) + (long long)o * a.y_stride + v0;
+        LgtVec<T, LGT_PER_LANE> raw[ITER];
+        uint32_t on[ITER];
+#pragma unroll
+        for (int t = 0; t < ITER; ++t) {
+            const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE;
+            raw[t] = lgt_load(dy, e, n - e);
+            on[t] = lgt_on8(a, mask_row, v0 + e, n - e);
+        }
+        const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
+        const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
+        if (a.history) lgt_count(a, o, v0, n, cnt);
+#pragma unroll
+        for (int t = 0; t < ITER; ++t) {
+            const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE, left = n - e;
+            if (left <= 0) break;
+            float g[LGT_PER_LANE];
+#pragma unroll
+            for (int k = 0; k < LGT_PER_LANE; ++k) {
+                g[k] = (on[t] >> k) & 1 ? (float)raw[t][k] * inv_tau : 0.f;
+                sum[t][k] += g[k];
+            }
+            if (!a.y) continue;
+            if (a.history) {
+                uint32_t c[LGT_PER_LANE];
+                *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(cnt + e);
+                *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(cnt + e + 4);
+                if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
+                    const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + v0;
+                    const LgtVec<T, LGT_PER_LANE> xs = lgt_load(x, e, left);
+#pragma unroll
+                    for (int k = 0; k < LGT_PER_LANE; ++k)
+                        if (c[k] && ((on[t] >> k) & 1)) g[k] *= (float)xs[k] > 0.f ? inv_rho : rho;
+                }
+            }
+            lgt_store(static_cast<T*>(a.y) + (long long)o * a.y_stride + v0, e, left, g);
+        }
+        if (a.history) __syncthreads();          // the counts are cleared for the next row
+    }
+    if (a.dbias) {
+        float* out = a.dbias + ((long long)part * a.bias_rows + r) * a.vocab + v0;
+#pragma unroll
+        for (int t = 0; t < ITER; ++t) {
+            const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE;
+            if (e < n) lgt_store(out, e, n - e, sum[t]);
         }
     }
 }
 
-// Gradient of the bias: one wavefront per (r, v) adds the rows o = r, r + R, ... and all i, each lane its own in order.
+// ---------------------------------------------------------------------------------------------- scores (inner > 1)
+// A workgroup's tile: `chunk` vocabulary entries with all their inner elements, which follow each other in memory.  What depends
+// on the entry alone stands in LDS: forward the sum of its additive terms, backward nothing, and two flags in the count.
+#define LGT_OFF 0x40000000u                    // replaces the count once it is used: the mask has the entry off
+
+__device__ __forceinline__ int lgt_entry(int e, float inv_inner) { return (int)((e + 0.5f) * inv_inner); }    // e < 2^22: exact
+
 template <typename T>
-__global__ __launch_bounds__(LGT_THREADS) void k_logits_bias_grad(LogitsArgs a, float* __restrict__ dbias) {
+__global__ __launch_bounds__(LGT_THREADS) void k_scores(LogitsArgs a) {
+    extern __shared__ __align__(16) uint32_t cnt[];
+    const int o = blockIdx.x / a.chunks, v0 = (blockIdx.x % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0);
+    float* add = reinterpret_cast<float*>(cnt + ((a.chunk + 3) & ~3));
+    const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
+    const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
+    const float pres = lgt_param(a.pres, a.pres_rows, a.pres_value, o), freq = lgt_param(a.freq, a.freq_rows, a.freq_value, o);
+    if (a.history) lgt_count(a, o, v0, n, cnt);
+    const float* bias = a.bias ? a.bias + (long long)(o % a.bias_rows) * a.vocab + v0 : nullptr;
+    const int mask_row = a.mask_type ? o % a.mask_rows : 0;
+    for (int v = threadIdx.x; v < n; v += LGT_THREADS) {
+        const uint32_t c = a.history ? cnt[v] : 0, times = c & ~LGT_SEEN;
+        float z = bias ? bias[v] : 0.f;
+        if (times) z -= (float)times * freq + pres;
+        add[v] = z;
+        cnt[v] = (c ? LGT_SEEN : 0) | (lgt_on(a, mask_row, v0 + v) ? 0 : LGT_OFF);
+    }
+    __syncthreads();
+    const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + (long long)v0 * a.inner;
+    T* y = static_cast<T*>(a.y) + (long long)o * a.y_stride + (long long)v0 * a.inner;
+    const int end = n * a.inner;
+    const float inv_inner = 1.f / (float)a.inner;
+    for (int e = threadIdx.x * LGT_PER_LANE; e < end; e += LGT_STRIDE) {
+        const LgtVec<T, LGT_PER_LANE> raw = lgt_load(x, e, end - e);
+        float z[LGT_PER_LANE];
+        int v = n == 1 ? 0 : lgt_entry(e, inv_inner), i = e - v * a.inner;
+#pragma unroll
+        for (int k = 0; k < LGT_PER_LANE; ++k) {
+            const uint32_t c = cnt[min(v, n - 1)];
+            z[k] = (float)raw[k];
+            if (c & LGT_SEEN) z[k] *= z[k] > 0.f ? inv_rho : rho;
+            z[k] = c & LGT_OFF ? a.masked_value : (z[k] + add[min(v, n - 1)]) * inv_tau;
+            if (++i == a.inner) { i = 0; ++v; }
+        }
+        lgt_store(y, e, end - e, z);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(LGT_THREADS) void k_scores_bwd(LogitsArgs a) {
+    extern __shared__ __align__(16) uint32_t cnt[];
+    float* tile = reinterpret_cast<float*>(cnt + ((a.chunk + 3) & ~3));        // only with dbias: chunk * inner elements
+    uint32_t at = blockIdx.x;
+    const int v0 = (int)(at % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0), end = n * a.inner;
+    at /= a.chunks;
+    const int r = (int)(at % a.bias_rows), part = (int)(at / a.bias_rows), many = a.rows / a.bias_rows;
+    const int first = (int)((long long)many * part / a.splits), last = (int)((long long)many * (part + 1) / a.splits);
+    const float inv_inner = 1.f / (float)a.inner;
+    // lanes that add one entry's elements: a power of two, so that they lie in one wavefront
+    int group = 1;
+    while (group < 64 && group * 2 * n <= LGT_THREADS) group *= 2;
+    const int mine = threadIdx.x / group, member = threadIdx.x % group;
+    float sum[LGT_PER_LANE] = {};
+    for (int q = first; q < last; ++q) {
+        const int o = r + q * a.bias_rows, mask_row = a.mask_type ? o % a.mask_rows : 0;
+        const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
+        const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
+        if (a.history) lgt_count(a, o, v0, n, cnt);
+        for (int v = threadIdx.x; v < n; v += LGT_THREADS)
+            cnt[v] = (a.history && cnt[v] ? LGT_SEEN : 0) | (lgt_on(a, mask_row, v0 + v) ? 0 : LGT_OFF);
+        __syncthreads();
+        const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + (long long)v0 * a.inner;
+        const T* dy = static_cast<const T*>(a.dy) + (long long)o * a.y_stride + (long long)v0 * a.inner;
+        T* dx = a.y ? static_cast<T*>(a.y) + (long long)o * a.y_stride + (long long)v0 * a.inner : nullptr;
+        for (int e = threadIdx.x * LGT_PER_LANE; e < end; e += LGT_STRIDE) {
+            const int left = end - e;
+            const LgtVec<T, LGT_PER_LANE> raw = lgt_load(dy, e, left);
+            float g[LGT_PER_LANE];
+            uint32_t c[LGT_PER_LANE], any = 0;
+            int v = n == 1 ? 0 : lgt_entry(e, inv_inner), i = e - v * a.inner;
+#pragma unroll
+            for (int k = 0; k < LGT_PER_LANE; ++k) {
+                c[k] = cnt[min(v, n - 1)];
+                any |= c[k];
+                g[k] = c[k] & LGT_OFF ? 0.f : (float)raw[k] * inv_tau;
+                if (++i == a.inner) { i = 0; ++v; }
+            }
+            if (a.dbias) lgt_store(tile, e, left, g);
+            if (dx) {
+                if (any & LGT_SEEN) {
+                    const LgtVec<T, LGT_PER_LANE> xs = lgt_load(x, e, left);
+#pragma unroll
+                    for (int k = 0; k < LGT_PER_LANE; ++k)
+                        if (c[k] == LGT_SEEN) g[k] *= (float)xs[k] > 0.f ? inv_rho : rho;
+                }
+                lgt_store(dx, e, left, g);
+            }
+        }
+        __syncthreads();
+        if (a.dbias) {
+            // entries mine, mine + 512 / group, ...: at most 8 passes, as a tile has at most 4096 elements in at most 2048 entries
+#pragma unroll
+            for (int p = 0; p < LGT_PER_LANE; ++p) {
+                const int v = mine + p * (LGT_THREADS / group);
+                float s = 0.f;
+                if (v < n)
+                    for (int i = member; i < a.inner; i += group) s += tile[v * a.inner + i];
+                for (int off = group >> 1; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
+                sum[p] += s;
+                if ((p + 1) * (LGT_THREADS / group) >= n) break;
+            }
+            __syncthreads();
+        }
+    }
+    if (a.dbias && member == 0) {
+        float* out = a.dbias + ((long long)part * a.bias_rows + r) * a.vocab + v0;
+#pragma unroll
+        for (int p = 0; p < LGT_PER_LANE; ++p) {
+            const int v = mine + p * (LGT_THREADS / group);
+            if (v < n) out[v] = sum[p];
+        }
+    }
+}
+
+// Gradient of the bias where an entry's inner elements exceed a tile: one wavefront per (r, v) adds the rows r, r + R, ... and
+// all i, each lane its own in order.
+template <typename T>
+__global__ __launch_bounds__(LGT_THREADS) void k_scores_bias_grad(LogitsArgs a, float* __restrict__ dbias) {
     const long long at = (long long)blockIdx.x * (LGT_THREADS / 64) + (threadIdx.x >> 6);
     if (at >= (long long)a.bias_rows * a.vocab) return;
     const int r = (int)(at / a.vocab), v = (int)(at % a.vocab), lane = threadIdx.x & 63;
-    const long long many = (long long)(a.rows / a.bias_rows) * a.inner;
     float sum = 0.f;
-    for (long long k = lane; k < many; k += 64) {
-        const int o = r + (int)(k / a.inner) * a.bias_rows;
+    for (int o = r; o < a.rows; o += a.bias_rows) {
         if (!lgt_on(a, a.mask_type ? o % a.mask_rows : 0, v)) continue;
+        const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
         const T* dy = static_cast<const T*>(a.dy) + (long long)o * a.y_stride + (long long)v * a.inner;
-        sum += (float)dy[k % a.inner] * (1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o));
+        for (int i = lane; i < a.inner; i += 64) sum += (float)dy[i] * inv_tau;
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
     if (lane == 0) dbias[at] = sum;
+}
+
+// The parts' sums of the bias gradient, added in order.
+__global__ __launch_bounds__(256) void k_logits_bias_sum(long long n, int splits, const float* __restrict__ part, float* __restrict__ dbias) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float sum = 0.f;
+    for (int p = 0; p < splits; ++p) sum += part[p * n + i];
+    dbias[i] = sum;
 }

@@ -1,5 +1,6 @@
 // C ABI of the logits operators: argument checks and launches.  The entry points are documented in include/gcn_uelb_hip.h.
 #include <algorithm>
+#include <cstdlib>
 
 #include "../../include/gcn_uelb_hip.h"
 #include "host.hpp"
@@ -10,6 +11,14 @@ namespace {
 int check_rows(const char* what, const void* p, long long n, long long rows) {
     if (p && (n < 1 || n > rows || rows % n)) return fail(-1, "gcn_logits: %lld rows of %s for %lld rows of logits", n, what, rows);
     return 0;
+}
+
+// Vocabulary of a workgroup of k_logits in strides of 4096 entries: more of them read the history less often, fewer make more
+// workgroups.
+int token_iterations(long long rows, long long vocab) {
+    const auto blocks = [&](long long it) { return rows * ((vocab + it * LGT_STRIDE - 1) / (it * LGT_STRIDE)); };
+    if (const char* e = tune_env("GCN_TUNE_LOGITS_IT")) return atoi(e);
+    return blocks(2) >= 1024 ? 2 : 1;
 }
 
 int fill_args(const gcn_logits_desc* d, LogitsArgs* a) {
@@ -47,32 +56,72 @@ int fill_args(const gcn_logits_desc* d, LogitsArgs* a) {
     a->rep = d->repetition_t; a->pres = d->presence_t; a->freq = d->frequency_t; a->temp = d->temperature_t;
     a->rep_value = d->repetition; a->pres_value = d->presence; a->freq_value = d->frequency; a->temp_value = d->temperature;
     a->masked_value = d->masked_value;
-    // about 1024 workgroups; a range of at least one pass of the workgroup and at most 16384 counts (64 KiB of LDS)
-    const long long want = (d->vocab * std::max(d->rows, 1ll) + 1023) / 1024;
-    a->chunk = (int)std::min<long long>(16384, std::max<long long>(LGT_STRIDE, (want + LGT_STRIDE - 1) / LGT_STRIDE * LGT_STRIDE));
+    if (d->inner == 1) {
+        a->chunk = LGT_STRIDE * token_iterations(d->rows, d->vocab);
+    } else {
+        a->chunk = (int)std::max(1ll, std::min(d->vocab, (long long)LGT_STRIDE / d->inner));
+    }
     a->chunks = (int)((d->vocab + a->chunk - 1) / a->chunk);
-    if (d->rows * a->chunks > 0x7fffffffll) return fail(-2, "gcn_logits: too many rows");
+    if (std::max(d->rows, 1ll) * a->chunks > 0x7fffffffll) return fail(-2, "gcn_logits: too many rows");
     return 0;
 }
 
-size_t lds_of(const LogitsArgs& a) { return a.history ? (size_t)std::min(a.chunk, a.vocab) * sizeof(uint32_t) : 0; }
+size_t lds_of(const LogitsArgs& a, bool with_add, bool with_tile) {
+    if (a.inner == 1) return a.history ? (size_t)a.chunk * sizeof(uint32_t) : 0;
+    return ((size_t)((a.chunk + 3) & ~3) + (with_add ? a.chunk : 0) + (with_tile ? LGT_STRIDE : 0)) * sizeof(uint32_t);
+}
 
-template <typename T, bool BACKWARD>
-int launch(const LogitsArgs& a, hipStream_t st) {
-    const size_t lds = lds_of(a);
-    GCN_PROF_PRE(BACKWARD ? "k_logits_bwd" : "k_logits");
-    k_logits<T, BACKWARD><<<(uint32_t)a.rows * a.chunks, LGT_THREADS, lds, st>>>(a);
+template <typename T>
+int launch_fwd(const LogitsArgs& a, hipStream_t st) {
+    const uint32_t blocks = (uint32_t)a.rows * a.chunks;
+    const size_t lds = lds_of(a, true, false);
+    GCN_PROF_PRE(a.inner == 1 ? "k_logits" : "k_scores");
+    if (a.inner > 1) k_scores<T><<<blocks, LGT_THREADS, lds, st>>>(a);
+    else if (a.chunk == LGT_STRIDE) k_logits<T, 1><<<blocks, LGT_THREADS, lds, st>>>(a);
+    else if (a.chunk == 2 * LGT_STRIDE) k_logits<T, 2><<<blocks, LGT_THREADS, lds, st>>>(a);
+    else k_logits<T, 4><<<blocks, LGT_THREADS, lds, st>>>(a);
     GCN_CHECK_LAUNCH("k_logits");
     return 0;
 }
 
+// Parts of the rows that share a bias row: about 1024 workgroups, but sums of the parts (written and read in fp32) of at most
+// an eighth of the gradient's bytes where that is more than a launch's worth.
+int splits_of(const LogitsArgs& a, bool want_bias, int type) {
+    const long long many = a.rows / a.bias_rows, per_part = (long long)a.chunks * a.bias_rows;
+    if (!want_bias) return (int)many;
+    long long splits = std::min(many, (1024 + per_part - 1) / per_part);
+    const long long data = (long long)a.rows * a.vocab * a.inner * (type == GCN_F32 ? 8 : 4), part = 8ll * a.bias_rows * a.vocab;
+    return (int)std::max(1ll, std::min(splits, std::max(data, 32ll << 20) / 8 / part));
+}
+bool tile_fits(const LogitsArgs& a) { return a.inner <= LGT_STRIDE; }
+
 template <typename T>
-int launch_bias(const LogitsArgs& a, float* dbias, hipStream_t st) {
-    const long long waves = (long long)a.bias_rows * a.vocab, blocks = (waves + LGT_THREADS / 64 - 1) / (LGT_THREADS / 64);
-    if (blocks > 0x7fffffffll) return fail(-2, "gcn_logits_process_bwd: bias too large");
-    GCN_PROF_PRE("k_logits_bias_grad");
-    k_logits_bias_grad<T><<<(uint32_t)blocks, LGT_THREADS, 0, st>>>(a, dbias);
-    GCN_CHECK_LAUNCH("k_logits_bias_grad");
+int launch_bwd(LogitsArgs a, float* dbias, int splits, float* parts, hipStream_t st) {
+    const bool by_tile = dbias && tile_fits(a);
+    a.splits = splits;
+    a.dbias = by_tile ? (splits > 1 ? parts : dbias) : nullptr;
+    if ((long long)a.chunks * a.bias_rows * splits > 0x7fffffffll) return fail(-2, "gcn_logits_process_bwd: too many rows");
+    const uint32_t blocks = (uint32_t)((long long)a.chunks * a.bias_rows * splits);
+    const size_t lds = lds_of(a, false, by_tile);
+    if (a.y || by_tile) {
+        GCN_PROF_PRE(a.inner == 1 ? "k_logits_bwd" : "k_scores_bwd");
+        if (a.inner > 1) k_scores_bwd<T><<<blocks, LGT_THREADS, lds, st>>>(a);
+        else if (a.chunk == LGT_STRIDE) k_logits_bwd<T, 1><<<blocks, LGT_THREADS, lds, st>>>(a);
+        else k_logits_bwd<T, 2><<<blocks, LGT_THREADS, lds, st>>>(a);
+        GCN_CHECK_LAUNCH("k_logits_bwd");
+    }
+    if (!dbias) return 0;
+    const long long n = (long long)a.bias_rows * a.vocab;
+    if (!by_tile) {
+        const long long blocks = (n + LGT_THREADS / 64 - 1) / (LGT_THREADS / 64);
+        GCN_PROF_PRE("k_scores_bias_grad");
+        k_scores_bias_grad<T><<<(uint32_t)blocks, LGT_THREADS, 0, st>>>(a, dbias);
+        GCN_CHECK_LAUNCH("k_scores_bias_grad");
+    } else if (splits > 1) {
+        GCN_PROF_PRE("k_logits_bias_sum");
+        k_logits_bias_sum<<<(uint32_t)((n + 255) / 256), 256, 0, st>>>(n, splits, parts, dbias);
+        GCN_CHECK_LAUNCH("k_logits_bias_sum");
+    }
     return 0;
 }
 
@@ -87,30 +136,36 @@ int gcn_logits_process(const gcn_logits_desc* d, const void* in, void* out, void
     if (!in || !out) return fail(-1, "gcn_logits_process: null pointer argument");
     a.x = in; a.y = out;
     hipStream_t st = (hipStream_t)stream;
-    if (d->type == GCN_F32) return launch<float, false>(a, st);
-    if (d->type == GCN_BF16) return launch<__bf16, false>(a, st);
-    return launch<_Float16, false>(a, st);
+    if (d->type == GCN_F32) return launch_fwd<float>(a, st);
+    if (d->type == GCN_BF16) return launch_fwd<__bf16>(a, st);
+    return launch_fwd<_Float16>(a, st);
 }
 
-int gcn_logits_process_bwd(const gcn_logits_desc* d, const void* in, const void* dout, void* din, float* dbias, void* stream) {
+size_t gcn_logits_bwd_ws_bytes(const gcn_logits_desc* d) {
+    LogitsArgs a;
+    if (fill_args(d, &a) || a.rows == 0 || !a.bias) return 0;
+    const int splits = splits_of(a, true, d->type);
+    return splits > 1 && tile_fits(a) ? (size_t)splits * a.bias_rows * a.vocab * sizeof(float) : 0;
+}
+
+int gcn_logits_process_bwd(const gcn_logits_desc* d, const void* in, const void* dout, void* din, float* dbias, void* ws, size_t ws_bytes,
+                           void* stream) {
     LogitsArgs a;
     if (int rc = fill_args(d, &a)) return rc;
     if (dbias && !d->bias) return fail(-1, "gcn_logits_process_bwd: gradient of a bias that is not there");
     if (a.rows == 0) return 0;
     if (!in || !dout || (!din && !dbias)) return fail(-1, "gcn_logits_process_bwd: null pointer argument");
+    const size_t need = dbias ? gcn_logits_bwd_ws_bytes(d) : 0;
+    if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 3))) return fail(-2, "gcn_logits_process_bwd: workspace too small");
     a.x = in; a.y = din; a.dy = dout;
+    if (!dbias) a.bias_rows = 1;
     // a repetition penalty of one changes no slope: the history is not needed
-    if (!a.rep && a.rep_value == 1.f) a.history = nullptr;
+    if (!din || (!a.rep && a.rep_value == 1.f)) a.history = nullptr;
+    const int splits = splits_of(a, dbias != nullptr, d->type);
     hipStream_t st = (hipStream_t)stream;
-    if (din) {
-        const int rc = d->type == GCN_F32 ? launch<float, true>(a, st) : d->type == GCN_BF16 ? launch<__bf16, true>(a, st) : launch<_Float16, true>(a, st);
-        if (rc) return rc;
-    }
-    if (dbias) {
-        const int rc = d->type == GCN_F32 ? launch_bias<float>(a, dbias, st) : d->type == GCN_BF16 ? launch_bias<__bf16>(a, dbias, st) : launch_bias<_Float16>(a, dbias, st);
-        if (rc) return rc;
-    }
-    return 0;
+    if (d->type == GCN_F32) return launch_bwd<float>(a, dbias, splits, (float*)ws, st);
+    if (d->type == GCN_BF16) return launch_bwd<__bf16>(a, dbias, splits, (float*)ws, st);
+    return launch_bwd<_Float16>(a, dbias, splits, (float*)ws, st);
 }
 
 }  // extern "C"

@@ -194,7 +194,9 @@ def _declare(lib):
     lib.gcn_logits_process.restype = c_int
     lib.gcn_logits_process.argtypes = [POINTER(LogitsDesc)] + [c_void_p] * 3
     lib.gcn_logits_process_bwd.restype = c_int
-    lib.gcn_logits_process_bwd.argtypes = [POINTER(LogitsDesc)] + [c_void_p] * 5
+    lib.gcn_logits_process_bwd.argtypes = [POINTER(LogitsDesc)] + [c_void_p] * 5 + [c_size_t, c_void_p]
+    lib.gcn_logits_bwd_ws_bytes.restype = c_size_t
+    lib.gcn_logits_bwd_ws_bytes.argtypes = [POINTER(LogitsDesc)]
 
 
 def load():

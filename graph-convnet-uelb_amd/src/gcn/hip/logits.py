@@ -172,9 +172,13 @@ class ProcessLogitsFn(torch.autograd.Function):
         dbias = torch.zeros(ctx.bias_shape, dtype=torch.float32, device=x.device) if want_bias and rules.rows == 0 else None
         if want_bias and dbias is None:
             dbias = torch.empty(ctx.bias_shape, dtype=torch.float32, device=x.device)
+        lib = L.load()
+        nbytes = lib.gcn_logits_bwd_ws_bytes(ctypes.byref(d)) if want_bias else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         with L.device_guard(x.device):
-            rc = L.load().gcn_logits_process_bwd(ctypes.byref(d), x.data_ptr(), dout.data_ptr(), None if dx is None else dx.data_ptr(),
-                                                 None if dbias is None else dbias.data_ptr(), L.stream_ptr(x.device))
+            rc = lib.gcn_logits_process_bwd(ctypes.byref(d), x.data_ptr(), dout.data_ptr(), None if dx is None else dx.data_ptr(),
+                                            None if dbias is None else dbias.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                                            L.stream_ptr(x.device))
         L.check(rc, "gcn_logits_process_bwd")
         return dx, dbias, None
 

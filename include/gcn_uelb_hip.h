@@ -360,7 +360,7 @@ int gcn_grad_norm(int n, int type, const void* const* grads, const long long* nu
  * bias: float [bias_rows][vocab] or NULL.  A row whose mask leaves nothing becomes masked_value throughout.
  * gcn_logits_process_bwd: dout and din have out_stride; din (NULL: not wanted) and dbias [bias_rows][vocab] (NULL likewise) are
  *   overwritten; both are 0 where the mask has v off, whatever in and dout hold there.  At x = 0 the slope is that of
- *   x < 0.  Sums are fp32 in a fixed order.
+ *   x < 0.  Sums are fp32 in a fixed order.  ws: gcn_logits_bwd_ws_bytes() bytes, needed with dbias only.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct gcn_logits_desc {
     long long rows, vocab, inner;
@@ -381,7 +381,9 @@ typedef struct gcn_logits_desc {
 } gcn_logits_desc;
 
 int gcn_logits_process(const gcn_logits_desc* d, const void* in, void* out, void* stream);
-int gcn_logits_process_bwd(const gcn_logits_desc* d, const void* in, const void* dout, void* din, float* dbias, void* stream);
+size_t gcn_logits_bwd_ws_bytes(const gcn_logits_desc* d);
+int gcn_logits_process_bwd(const gcn_logits_desc* d, const void* in, const void* dout, void* din, float* dbias, void* ws,
+                           size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -95,8 +95,8 @@ def test_c_entry_points_refuse_without_touching_memory():
     for big in (dict(vocab=1 << 31, out_stride=1 << 31), dict(vocab=1 << 20, inner=1 << 11, out_stride=1 << 31), dict(rows=1 << 31)):
         assert call(**big) == -2, big
     d = L.LogitsDesc(**ok)
-    assert lib.gcn_logits_process_bwd(ctypes.byref(d), None, None, None, 16, None) == -1 and b"bias" in lib.gcn_last_error()
-    assert lib.gcn_logits_process_bwd(ctypes.byref(d), 16, 16, None, None, None) == -1
+    assert lib.gcn_logits_process_bwd(ctypes.byref(d), None, None, None, 16, None, 0, None) == -1 and b"bias" in lib.gcn_last_error()
+    assert lib.gcn_logits_process_bwd(ctypes.byref(d), 16, 16, None, None, None, 0, None) == -1
 
 
 def test_oracle_gradient_against_differences():
@@ -115,3 +115,17 @@ def test_oracle_gradient_against_differences():
             step[k] = 1e-6
             args = [(x + step, b), (x - step, b)] if at == 0 else [(x, b + step), (x, b - step)]
             assert abs((f(*args[0]) - f(*args[1])) / 2e-6 - grad[k]) < 1e-6
+
+
+def test_workspace_of_the_bias_gradient():
+    lib = L.load()
+    ok = dict(vocab=1000, inner=1, in_stride=1000, out_stride=1000, history_rows=1, mask_rows=1, repetition_rows=1, presence_rows=1,
+              frequency_rows=1, temperature_rows=1, type=0, repetition=1.0, temperature=1.0)
+    ws = lambda **k: lib.gcn_logits_bwd_ws_bytes(ctypes.byref(L.LogitsDesc(**{**ok, **k})))
+    assert ws(rows=8) == 0                                         # no bias
+    assert ws(rows=8, bias=16, bias_rows=8) == 0                   # a row of its own for each: nothing to add
+    shared = ws(rows=2000, bias=16, bias_rows=1)
+    assert shared > 0 and shared % 4000 == 0                       # whole rows of sums
+    assert ws(rows=2, vocab=4, inner=100000, out_stride=400000, bias=16, bias_rows=1) == 0
+    d = L.LogitsDesc(**{**ok, "rows": 2000, "bias": 16, "bias_rows": 1})
+    assert lib.gcn_logits_process_bwd(ctypes.byref(d), 16, 16, 16, 16, None, 0, None) == -2 and b"workspace" in lib.gcn_last_error()
