@@ -18,48 +18,7 @@ import torch
 from . import lib as L
 
 STATE8_BLOCK = 128
-_TYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_numel, _data_ptr, _get_device, _is_contiguous = (torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.get_device,
-                                                  torch.Tensor.is_contiguous)
-
-
-def _table(tensors):
-    return (ctypes.c_void_p * len(tensors))(*map(_data_ptr, tensors))
-
-
-def _same_list(name, tensors, numels, dtypes):
-    """Checks one list of a call: as many tensors as parameters, of these sizes and types, contiguous."""
-    if len(tensors) != len(numels):
-        raise ValueError(f"{len(tensors)} tensors in {name} for {len(numels)} parameters")
-    if list(map(_numel, tensors)) != numels:
-        raise ValueError(f"the tensors in {name} do not have the parameters' sizes")
-    got = {t.dtype for t in tensors}
-    if not got <= dtypes:
-        raise TypeError(f"{name} holds {', '.join(map(str, got - dtypes))} (expected {', '.join(map(str, dtypes))})")
-    if not all(map(_is_contiguous, tensors)):
-        raise ValueError(f"{name} needs contiguous tensors")
-
-
-def _one_device(lists):
-    """The device that all tensors are on."""
-    found = set(itertools.chain.from_iterable(map(_get_device, ts) for ts in lists if ts))
-    if -1 in found:
-        L.require_cuda(next(t for ts in lists if ts for t in ts if not t.is_cuda), "tensor")
-    if len(found) != 1:
-        raise ValueError("the tensors of one call are on one GPU")
-    return next(t for ts in lists if ts for t in ts).device
-
-
-def _scalar(t, name, device):
-    """A number in device memory that a kernel reads."""
-    if t is None:
-        return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1:
-        raise TypeError(f"{name} is a float32 tensor of one element")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the tensors are on {device}")
-    return t.data_ptr()
-
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 def _blocks_of(n):
     return -(-n // STATE8_BLOCK)
@@ -76,49 +35,10 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0
     bits of the 8-bit states' rounding, as does a tensor's place in the list.  hyper: what ``adamw_advance_`` filled, in place
     of step and of the numbers from lr on; a step that is captured into a graph needs it.  The tensors of a call must not
     overlap."""
-    eight = exp_avg_exps is not None
-    if eight != (exp_avg_sq_exps is not None):
-        raise ValueError("exp_avg_exps and exp_avg_sq_exps go together")
     if hyper is None and (int(step) != step or step < 1):
         raise ValueError(f"step counts from 1, got {step}")
-    kinds = {p.dtype for p in params}
-    if len(kinds) > 1 or not kinds <= _TYPE_ID.keys():
-        raise TypeError(f"parameters of one type per call (float32, bfloat16 or float16), got {', '.join(map(str, kinds))}")
-    numels = list(map(_numel, params))
-    _same_list("params", params, numels, kinds)
-    _same_list("grads", grads, numels, kinds)
-    half = bool(kinds) and torch.float32 not in kinds
-    if bool(params) and half != (masters is not None):
-        raise ValueError("master copies go with 16-bit parameters, and only with them")
-    state = {torch.uint8} if eight else {torch.float32}
-    _same_list("exp_avgs", exp_avgs, numels, state)
-    _same_list("exp_avg_sqs", exp_avg_sqs, numels, state)
-    lists = [params, grads, exp_avgs, exp_avg_sqs]
-    if half:
-        _same_list("masters", masters, numels, {torch.float32})
-        lists.append(masters)
-    if eight:
-        blocks = list(map(_blocks_of, numels))
-        _same_list("exp_avg_exps", exp_avg_exps, blocks, state)
-        _same_list("exp_avg_sq_exps", exp_avg_sq_exps, blocks, state)
-        lists += [exp_avg_exps, exp_avg_sq_exps]
-    desc = L.AdamWDesc(n=len(numels), param_type=_TYPE_ID[next(iter(kinds))] if kinds else 0, state_bits=8 if eight else 32,
-                       first_tensor=first_tensor, lr=lr, beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay,
-                       step=0 if hyper is not None else int(step), seed=seed)
-    lib = L.load()
-    if not numels:
-        return
-    dev = _one_device(lists)
-    if hyper is None and torch.cuda.is_current_stream_capturing():
-        raise L.GcnHipError("a captured step would repeat its step count: pass hyper (adamw_advance_)")
-    if hyper is not None and (hyper.device != dev or hyper.dtype != torch.uint8 or hyper.numel() < lib.gcn_adamw_hyper_bytes()):
-        raise ValueError("hyper is what adamw_hyper returned, on the tensors' device")
-    scale, clip = _scalar(grad_scale, "grad_scale", dev), _scalar(clip_coef, "clip_coef", dev)
-    with L.device_guard(dev):
-        rc = lib.gcn_adamw_step(ctypes.byref(desc), *map(_table, lists[:2]), _table(masters) if half else None, *map(_table, lists[2:4]),
-                                *(map(_table, lists[-2:]) if eight else (None, None)), (ctypes.c_longlong * len(numels))(*numels),
-                                scale, clip, None if hyper is None else hyper.data_ptr(), L.stream_ptr(dev))
-    L.check(rc, "gcn_adamw_step")
+    L.binding().adamw_step(params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_exps, exp_avg_sq_exps, int(step), lr, betas[0], betas[1], eps,
+                           weight_decay, seed, first_tensor, grad_scale, clip_coef, hyper)
 
 
 def adamw_hyper(device):
@@ -139,33 +59,17 @@ def adamw_advance_(step, hyper, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_deca
     on_device = isinstance(lr, torch.Tensor)
     desc = L.AdamWDesc(n=0, state_bits=32, lr=0.0 if on_device else lr, beta1=betas[0], beta2=betas[1], eps=eps,
                        weight_decay=weight_decay, seed=seed)
-    lr_ptr = _scalar(lr, "lr", dev) if on_device else None
+    if on_device and (lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev):
+        raise TypeError("lr on the device is a float32 tensor of one element, where step is")
     with L.device_guard(dev):
-        rc = lib.gcn_adamw_advance(ctypes.byref(desc), step.data_ptr(), lr_ptr, hyper.data_ptr(), L.stream_ptr(dev))
+        rc = lib.gcn_adamw_advance(ctypes.byref(desc), step.data_ptr(), lr.data_ptr() if on_device else None, hyper.data_ptr(), L.stream_ptr(dev))
     L.check(rc, "gcn_adamw_advance")
 
 
 def grad_norm(grads, *, max_norm=None, grad_scale=None):
     """(norm, coefficient): the 2-norm of all gradients together, times grad_scale, and min(1, max_norm / (norm + 1e-6)) or None
     without max_norm, as scalars on the device.  The gradients are of one type and on one GPU and are not changed."""
-    kinds = {g.dtype for g in grads}
-    if len(kinds) != 1 or not kinds <= _TYPE_ID.keys():
-        raise TypeError(f"gradients of one type per call (float32, bfloat16 or float16), got {', '.join(map(str, kinds)) or 'none'}")
-    if max_norm is not None and not max_norm >= 0:
-        raise ValueError(f"max_norm is not negative, got {max_norm}")
-    numels = list(map(_numel, grads))
-    _same_list("grads", grads, numels, kinds)
-    lib = L.load()
-    dev = _one_device([grads])
-    scale = _scalar(grad_scale, "grad_scale", dev)
-    sizes = (ctypes.c_longlong * len(numels))(*numels)
-    ws = torch.empty(lib.gcn_grad_norm_ws_bytes(len(numels), sizes), dtype=torch.uint8, device=dev)
-    out = torch.empty(2, dtype=torch.float32, device=dev)
-    with L.device_guard(dev):
-        rc = lib.gcn_grad_norm(len(numels), _TYPE_ID[next(iter(kinds))], _table(grads), sizes, scale,
-                               1.0 if max_norm is None else float(max_norm), out.data_ptr(), ws.data_ptr(), ws.numel(), L.stream_ptr(dev))
-    L.check(rc, "gcn_grad_norm")
-    return out[0], None if max_norm is None else out[1]
+    return L.binding().grad_norm(grads, max_norm, grad_scale)
 
 
 # ------------------------------------------------------------------------------------------------ 8-bit states
@@ -261,7 +165,7 @@ class FusedAdamW(torch.optim.Optimizer):
         L.require_cuda(p, "parameter")
         if p.grad.is_sparse:
             raise RuntimeError("FusedAdamW does not support sparse gradients")
-        if p.dtype not in _TYPE_ID:
+        if p.dtype not in _TYPES:
             raise TypeError(f"FusedAdamW updates float32, bfloat16 and float16 parameters, got {p.dtype}")
         if not p.is_contiguous():
             raise RuntimeError("FusedAdamW needs contiguous parameters")

@@ -15,6 +15,7 @@ import torch
 
 _PKG_ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), "..", "..", ".."))
 LIB_PATH = os.environ.get("GCN_UELB_LIB") or os.path.join(_PKG_ROOT, "lib", "libgcn_uelb_hip.so")
+BINDING_PATH = os.path.join(_PKG_ROOT, "lib", "gcn_uelb_torch.so")
 ABI_VERSION = 4
 MAX_H = 320
 LAYER_NPARAMS = 12
@@ -32,20 +33,27 @@ BUILD_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
 
 
 def source_files():
-    """The files the library is built from: csrc/*.hip, csrc/*.hpp and the public header."""
+    """The files the library and its torch binding are built from: csrc/*.hip, *.hpp, *.cpp and the public header."""
     csrc = os.path.join(_PKG_ROOT, "csrc")
-    files = sorted(os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".hip", ".hpp")))
+    files = sorted(os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".hip", ".hpp", ".cpp")))
     files.append(os.path.abspath(os.path.join(_PKG_ROOT, "..", "include", "gcn_uelb_hip.h")))
     return files
 
 
 def build_commands(hipcc, out):
-    """One compile command per translation unit (csrc/*.hip; they are independent of each other) and the link command."""
+    """One compile command per translation unit (csrc/*.hip; they are independent of each other) and the torch binding's, then
+    the link command."""
+    import sysconfig
     obj_dir = os.path.join(_PKG_ROOT, "build")
     os.makedirs(obj_dir, exist_ok=True)
     units = [f for f in source_files() if f.endswith(".hip")]
     objs = [os.path.join(obj_dir, os.path.basename(f)[:-4] + ".o") for f in units]
-    return ([[hipcc, *BUILD_FLAGS, "-c", "-o", o, f] for f, o in zip(units, objs)],
+    root = os.path.dirname(torch.__file__)
+    binding = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{root}/include",
+               f"-I{root}/include/torch/csrc/api/include", "-I" + os.path.join(os.path.dirname(hipcc), "..", "include"),
+               "-I" + sysconfig.get_paths()["include"], "-o", BINDING_PATH, os.path.join(_PKG_ROOT, "csrc", "torch_binding.cpp"),
+               f"-L{root}/lib", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+    return ([[hipcc, *BUILD_FLAGS, "-c", "-o", o, f] for f, o in zip(units, objs)] + [binding],
             [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out, *objs])
 
 
@@ -224,6 +232,31 @@ def load():
             raise GcnHipError(f"ABI mismatch: library {lib.gcn_abi_version()} vs binding {ABI_VERSION}")
         _lib = lib
     return _lib
+
+
+_binding = None
+_BOUND = ("gcn_last_error", "gcn_adamw_step", "gcn_adamw_hyper_bytes", "gcn_grad_norm_ws_bytes", "gcn_grad_norm", "gcn_logits_process",
+          "gcn_logits_bwd_ws_bytes", "gcn_logits_process_bwd")
+
+
+def binding():
+    """The native module that takes torch tensors (csrc/torch_binding.cpp), with the library's functions handed to it (once)."""
+    global _binding
+    if _binding is None:
+        import importlib.util
+        lib = load()
+        if not os.path.exists(BINDING_PATH):
+            raise GcnHipError(f"{BINDING_PATH} not found: build it with `python __graft_entry__.py build`; there is no fallback path")
+        stamp = BINDING_PATH + ".srchash"
+        if not os.path.exists(stamp) or open(stamp).read().strip() != source_hash():
+            raise GcnHipError(f"{BINDING_PATH} was built from other sources than those in {_PKG_ROOT}/csrc: rebuild it with "
+                              f"`python __graft_entry__.py build`")
+        spec = importlib.util.spec_from_file_location("gcn_uelb_torch", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in _BOUND}, GcnHipError)
+        _binding = module
+    return _binding
 
 
 def layer_plan(B, V, C, H):

@@ -7,7 +7,7 @@ import torch
 
 from oracle import logits_oracle as O
 from src.gcn.hip import lib as L
-from src.gcn.hip.logits import _row_stride, pack_mask, process_logits
+from src.gcn.hip.logits import pack_mask, process_logits
 
 X = torch.zeros(2, 3, 10)
 
@@ -65,13 +65,14 @@ def test_pack_mask():
 
 
 def test_row_stride():
+    stride = L.binding().row_stride
     x = torch.zeros(4, 6, 10)
-    assert _row_stride(x, 2) == 10 and _row_stride(x, 1) == 60 and _row_stride(x, 0) == 240
-    assert _row_stride(x[:, :, :7], 2) == 10 and _row_stride(x[:, :, ::2], 2) is None
-    assert _row_stride(x[:, :3], 2) is None                       # rows not evenly spaced
-    assert _row_stride(x[:1, :3], 2) == 10 and _row_stride(x[:, :1], 2) == 60
-    assert _row_stride(torch.zeros(10).expand(4, 10), 1) == 0
-    assert _row_stride(x.transpose(0, 1), 2) is None
+    assert stride(x, 2) == 10 and stride(x, 1) == 60 and stride(x, 0) == 240
+    assert stride(x[:, :, :7], 2) == 10 and stride(x[:, :, ::2], 2) == -1
+    assert stride(x[:, :3], 2) == -1                              # rows not evenly spaced
+    assert stride(x[:1, :3], 2) == 10 and stride(x[:, :1], 2) == 60
+    assert stride(torch.zeros(10).expand(4, 10), 1) == 0
+    assert stride(x.transpose(0, 1), 2) == -1
 
 
 def test_c_entry_points_refuse_without_touching_memory():
