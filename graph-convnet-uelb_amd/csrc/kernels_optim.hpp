@@ -24,25 +24,31 @@
 #include <stdint.h>
 
 #define OPT_BLOCK 128                // elements that share an exponent byte
-#define OPT_WORDS 432                // 64-bit words for the tensors' table in the kernel arguments (3.4 of 4 KiB)
-#define OPT_MAX_TENSORS 64           // tensors of one launch: one lane of a wavefront looks up each
+#define OPT_ENTRIES 648              // 48-bit entries of the tensors' table in the kernel arguments (3.8 of 4 KiB)
 #define OPT_THREADS 256
 #define OPT_PER_LANE 8               // consecutive elements of a lane
 #define OPT_STRIDE (OPT_THREADS * OPT_PER_LANE)
-#define OPT_VEC (1ull << 63)         // flag in a tensor's element count: every pointer allows 16-byte (codes: 8-byte) access
+#define OPT_VEC (1ull << 47)         // flag in a tensor's element count: every pointer allows 16-byte (codes: 8-byte) access
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
-// Words of tensor k: its element count (with OPT_VEC), then its pointers: parameter, gradient, exp_avg, exp_avg_sq
-// [, master] [, exponent bytes of exp_avg, of exp_avg_sq].  first[k]: the launch's first workgroup of tensor k.
+// The tensors of a launch, in its arguments: a step over small tensors is as long as its launches, so that as many tensors as
+// possible share one.  Entry f of tensor k is number f * cap + k: 0 its element count (with OPT_VEC), then its addresses
+// (user addresses have 47 bits): parameter, gradient, exp_avg, exp_avg_sq [, master] [, exponent bytes of exp_avg, of
+// exp_avg_sq].  129 tensors with fp32 states fit, 92 with 8-bit ones, 324 gradients.
 struct OptTable {
-    uint64_t w[OPT_WORDS];
-    uint32_t first[OPT_MAX_TENSORS];
+    uint32_t lo[OPT_ENTRIES];
+    uint32_t hi[OPT_ENTRIES / 2];    // two 16-bit halves
     uint32_t ordinal;                // number of the first tensor (enters the hash)
-    int n, stride;                   // tensors, words per tensor
+    int n, cap;                      // tensors, places
+    uint32_t span, span_log2;        // elements of a workgroup
 };
+__device__ __forceinline__ uint64_t opt_entry(const OptTable& t, int field, int k) {
+    const int e = field * t.cap + k;
+    return ((uint64_t)(t.hi[e >> 1] >> (16 * (e & 1)) & 0xFFFFu) << 32) | t.lo[e];
+}
 
 struct AdamwHyper {
     float b1, omb1, b2, omb2, eps, decay, step_size, inv_sqrt_bc2;
@@ -73,12 +79,32 @@ __device__ __host__ inline AdamwHyper opt_hyper(double lr, double b1, double b2,
     return h;
 }
 
-// The tensor that this workgroup works on: the last one whose first workgroup is not behind it.  One lane looks up each
-// tensor, so that the search is one memory access deep.
-__device__ __forceinline__ int opt_find(const OptTable& t) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t f = lane < t.n ? t.first[lane] : 0xFFFFFFFFu;
-    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(f <= blockIdx.x)) - 1);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t opt_scan_step(uint32_t x) {
+    return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+// The tensor that this workgroup works on and which of its units: a lane adds the units of a few tensors, a scan over the
+// wavefront places them (no table of first workgroups, whose room goes to more tensors).
+__device__ __forceinline__ int opt_find(const OptTable& t, uint32_t* unit) {
+    const int lane = threadIdx.x & 63, per = (t.n + 63) >> 6;
+    const auto units = [&](int k) { return (uint32_t)(((opt_entry(t, 0, k) & ~OPT_VEC) + t.span - 1) >> t.span_log2); };
+    uint32_t mine = 0;
+    for (int j = 0; j < per; ++j)
+        if (lane * per + j < t.n) mine += units(lane * per + j);
+    uint32_t up_to = mine;                                          // sum over this lane and those before it
+    up_to = opt_scan_step<0x111, 0xf>(up_to);
+    up_to = opt_scan_step<0x112, 0xf>(up_to);
+    up_to = opt_scan_step<0x114, 0xf>(up_to);
+    up_to = opt_scan_step<0x118, 0xf>(up_to);
+    up_to = opt_scan_step<0x142, 0xa>(up_to);
+    up_to = opt_scan_step<0x143, 0xc>(up_to);
+    const uint64_t has = __ballot(blockIdx.x >= up_to - mine && blockIdx.x < up_to);
+    const int owner = __builtin_ctzll(has);
+    uint32_t rest = blockIdx.x - (uint32_t)__builtin_amdgcn_readlane((int)(up_to - mine), owner);
+    int k = __builtin_amdgcn_readfirstlane(owner * per);
+    for (uint32_t u; rest >= (u = units(k)); ++k) rest -= u;
+    *unit = rest;
+    return k;
 }
 
 // Eight elements at i: a 16-byte access for each four (16-bit types: eight) where `vec`, single ones otherwise and
@@ -172,26 +198,26 @@ __device__ __forceinline__ uint32_t opt_code(float scaled, uint32_t random16) {
     return min(c, 126u);
 }
 
-template <int UNITS, typename P, bool MASTER, bool EIGHT>
+template <typename P, bool MASTER, bool EIGHT>
 __global__ __launch_bounds__(OPT_THREADS) void k_adamw(OptTable t, AdamwHyper by_value, const AdamwHyper* __restrict__ in_memory,
                                                        const float* __restrict__ grad_scale, const float* __restrict__ clip) {
 #pragma clang fp contract(off)
-    const int k = opt_find(t);
-    const uint64_t* w = t.w + k * t.stride;
-    const uint64_t n = w[0] & ~OPT_VEC;
-    const bool vec = (w[0] & OPT_VEC) != 0;
-    P* p = (P*)w[1];
-    const P* g = (const P*)w[2];
-    float* master = MASTER ? (float*)w[5] : nullptr;
+    uint32_t unit;
+    const int k = opt_find(t, &unit);
+    const uint64_t size = opt_entry(t, 0, k), n = size & ~OPT_VEC;
+    const bool vec = (size & OPT_VEC) != 0;
+    P* p = (P*)opt_entry(t, 1, k);
+    const P* g = (const P*)opt_entry(t, 2, k);
+    void *m_at = (void*)opt_entry(t, 3, k), *v_at = (void*)opt_entry(t, 4, k);
+    float* master = MASTER ? (float*)opt_entry(t, 5, k) : nullptr;
     uint8_t *exp_m = nullptr, *exp_v = nullptr;
-    if constexpr (EIGHT) { exp_m = (uint8_t*)w[MASTER ? 6 : 5]; exp_v = (uint8_t*)w[MASTER ? 7 : 6]; }
+    if constexpr (EIGHT) { exp_m = (uint8_t*)opt_entry(t, MASTER ? 6 : 5, k); exp_v = (uint8_t*)opt_entry(t, MASTER ? 7 : 6, k); }
     const AdamwHyper h = in_memory ? *in_memory : by_value;
     const float s = (grad_scale ? *grad_scale : 1.f) * (clip ? *clip : 1.f);
     const uint32_t key = EIGHT ? opt_mix(h.key ^ ((t.ordinal + (uint32_t)k) * 0x85EBCA6BU)) : 0;
-    const uint64_t start = (uint64_t)(blockIdx.x - t.first[k]) * (UNITS * OPT_STRIDE) + threadIdx.x * OPT_PER_LANE;
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-        const uint64_t i = start + u * OPT_STRIDE;
+    const uint64_t start = (uint64_t)unit << t.span_log2;
+    for (uint32_t at = 0; at < t.span; at += OPT_STRIDE) {
+        const uint64_t i = start + at + threadIdx.x * OPT_PER_LANE;
         const int left = i < n ? (int)min(n - i, (uint64_t)OPT_PER_LANE) : 0;
         // a wavefront without elements leaves; one with some keeps all its lanes for the blocks' maxima
         if (__ballot(left > 0) == 0) break;
@@ -199,22 +225,21 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adamw(OptTable t, AdamwHyper by
         opt_load(g, i, left, vec, gi);
         if constexpr (MASTER) opt_load(master, i, left, vec, pi);
         else opt_load(p, i, left, vec, pi);
-        uint32_t cm[2], cr[2];
         if constexpr (EIGHT) {
-            opt_load_codes((const uint8_t*)w[3], i, left, vec, cm);
-            opt_load_codes((const uint8_t*)w[4], i, left, vec, cr);
-            const uint64_t b = i / OPT_BLOCK;
-            const float sm = opt_pow2(left ? exp_m[b] : 0), sr = opt_pow2(left ? exp_v[b] : 0);
+            uint32_t cm[2], cr[2];
+            opt_load_codes((const uint8_t*)m_at, i, left, vec, cm);
+            opt_load_codes((const uint8_t*)v_at, i, left, vec, cr);
+            const float sm = opt_pow2(left ? exp_m[i / OPT_BLOCK] : 0), sr = opt_pow2(left ? exp_v[i / OPT_BLOCK] : 0);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], false), b2 = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], true);
+                const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], true);
                 const auto c = __builtin_amdgcn_cvt_pk_f32_fp8(cr[q], false), d = __builtin_amdgcn_cvt_pk_f32_fp8(cr[q], true);
-                m[4 * q] = a[0] * sm; m[4 * q + 1] = a[1] * sm; m[4 * q + 2] = b2[0] * sm; m[4 * q + 3] = b2[1] * sm;
+                m[4 * q] = a[0] * sm; m[4 * q + 1] = a[1] * sm; m[4 * q + 2] = b[0] * sm; m[4 * q + 3] = b[1] * sm;
                 r[4 * q] = c[0] * sr; r[4 * q + 1] = c[1] * sr; r[4 * q + 2] = d[0] * sr; r[4 * q + 3] = d[1] * sr;
             }
         } else {
-            opt_load((const float*)w[3], i, left, vec, m);
-            opt_load((const float*)w[4], i, left, vec, r);
+            opt_load((const float*)m_at, i, left, vec, m);
+            opt_load((const float*)v_at, i, left, vec, r);
         }
         uint32_t top_m = 0, top_r = 0;
 #pragma unroll
@@ -228,23 +253,30 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adamw(OptTable t, AdamwHyper by
             pi[e] = pi[e] * h.decay - h.step_size * change;
             r[e] = EIGHT ? root : v;
             if constexpr (EIGHT) {
-                const uint32_t bm = __builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu, br = __builtin_bit_cast(uint32_t, root) & 0x7FFFFFFFu;
-                if (e < left) {
-                    top_m = max(top_m, bm < 0x7F800000u ? bm : 0u);
-                    top_r = max(top_r, br < 0x7F800000u ? br : 0u);
-                }
+                top_m = max(top_m, __builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu);
+                top_r = max(top_r, __builtin_bit_cast(uint32_t, root) & 0x7FFFFFFFu);
             }
         }
         if constexpr (MASTER) opt_store(master, i, left, vec, pi);
         opt_store(p, i, left, vec, pi);
         if constexpr (EIGHT) {
+            if (max(top_m, top_r) >= 0x7F800000u) {              // a value that is not finite: the largest of the others
+                top_m = top_r = 0;
+#pragma unroll
+                for (int e = 0; e < OPT_PER_LANE; ++e) {
+                    const uint32_t bm = __builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu, br = __builtin_bit_cast(uint32_t, r[e]) & 0x7FFFFFFFu;
+                    top_m = max(top_m, bm < 0x7F800000u ? bm : 0u);
+                    top_r = max(top_r, br < 0x7F800000u ? br : 0u);
+                }
+            }
+            // elements behind the end are zeros (or not finite, by a scale that is not) and change no maximum
             const uint32_t em = opt_exponent(opt_max16(top_m)), er = opt_exponent(opt_max16(top_r));
             const float um = opt_pow2(254 - em), ur = opt_pow2(254 - er);
-            cm[0] = cm[1] = cr[0] = cr[1] = 0;
+            uint32_t cm[2] = {0, 0}, cr[2] = {0, 0};
 #pragma unroll
             for (int e = 0; e < OPT_PER_LANE; ++e) {
-                const uint64_t at = i + e;
-                const uint32_t random = opt_mix(key ^ (uint32_t)at ^ ((uint32_t)(at >> 32) * 0xC2B2AE35U));
+                const uint64_t place = i + e;
+                const uint32_t random = opt_mix(key ^ (uint32_t)place ^ ((uint32_t)(place >> 32) * 0xC2B2AE35U));
                 uint32_t a = opt_code(__builtin_fabsf(m[e]) * um, random & 0xFFFFu);
                 a |= m[e] < 0.f ? 128u : 0u;
                 uint32_t b = opt_code(r[e] * ur, random >> 16);
@@ -252,15 +284,15 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adamw(OptTable t, AdamwHyper by
                 cm[e >> 2] |= a << (8 * (e & 3));
                 cr[e >> 2] |= b << (8 * (e & 3));
             }
-            opt_store_codes((uint8_t*)w[3], i, left, vec, cm);
-            opt_store_codes((uint8_t*)w[4], i, left, vec, cr);
+            opt_store_codes((uint8_t*)m_at, i, left, vec, cm);
+            opt_store_codes((uint8_t*)v_at, i, left, vec, cr);
             if ((threadIdx.x & 15) == 0 && left > 0) {
                 exp_m[i / OPT_BLOCK] = (uint8_t)em;
                 exp_v[i / OPT_BLOCK] = (uint8_t)er;
             }
         } else {
-            opt_store((float*)w[3], i, left, vec, m);
-            opt_store((float*)w[4], i, left, vec, r);
+            opt_store((float*)m_at, i, left, vec, m);
+            opt_store((float*)v_at, i, left, vec, r);
         }
     }
 }
@@ -276,25 +308,27 @@ __global__ void k_adamw_advance(long long* __restrict__ step, const float* __res
 // Sum of squares of one unit of elements per workgroup, in double precision: no overflow or underflow of squares of finite
 // gradients, and no rounding that shows.  Every partial sum has a place of its own and the second kernel adds them in a fixed
 // order, so that equal gradients give equal bits.
-template <int UNITS, typename P>
+#define OPT_NORM_UNITS 4             // strides of a workgroup, all of them on the way at once
+template <typename P>
 __global__ __launch_bounds__(OPT_THREADS) void k_grad_norm(OptTable t, double* __restrict__ part) {
     __shared__ double wave_sum[OPT_THREADS / 64];
-    const int k = opt_find(t);
-    const uint64_t* w = t.w + k * t.stride;
-    const uint64_t n = w[0] & ~OPT_VEC;
-    const bool vec = (w[0] & OPT_VEC) != 0;
-    const P* g = (const P*)w[1];
-    const uint64_t start = (uint64_t)(blockIdx.x - t.first[k]) * (UNITS * OPT_STRIDE) + threadIdx.x * OPT_PER_LANE;
+    uint32_t unit;
+    const int k = opt_find(t, &unit);
+    const uint64_t size = opt_entry(t, 0, k), n = size & ~OPT_VEC;
+    const bool vec = (size & OPT_VEC) != 0;
+    const P* g = (const P*)opt_entry(t, 1, k);
+    const uint64_t start = (uint64_t)unit * (OPT_NORM_UNITS * OPT_STRIDE) + threadIdx.x * OPT_PER_LANE;
     double sum = 0.0;
-#pragma unroll 4
-    for (int u = 0; u < UNITS; ++u) {
-        const uint64_t i = start + u * OPT_STRIDE;
-        const int left = i < n ? (int)min(n - i, (uint64_t)OPT_PER_LANE) : 0;
-        float x[OPT_PER_LANE];
-        opt_load(g, i, left, vec, x);
+    float x[OPT_NORM_UNITS][OPT_PER_LANE];
 #pragma unroll
-        for (int e = 0; e < OPT_PER_LANE; ++e) sum += (double)x[e] * (double)x[e];
+    for (int u = 0; u < OPT_NORM_UNITS; ++u) {
+        const uint64_t i = start + u * OPT_STRIDE;
+        opt_load(g, i, i < n ? (int)min(n - i, (uint64_t)OPT_PER_LANE) : 0, vec, x[u]);
     }
+#pragma unroll
+    for (int u = 0; u < OPT_NORM_UNITS; ++u)
+#pragma unroll
+        for (int e = 0; e < OPT_PER_LANE; ++e) sum += (double)x[u][e] * (double)x[u][e];
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
     if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = sum;
@@ -311,6 +345,7 @@ __global__ __launch_bounds__(1024) void k_grad_norm_final(int n, const double* _
                                                           double max_norm, float* __restrict__ out) {
     __shared__ double wave_sum[16];
     double sum = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < n; i += 1024) sum += part[i];
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);

@@ -9,16 +9,31 @@
 
 namespace {
 
-constexpr int kAdamwUnits = 2;       // 2048-element strides of a workgroup of k_adamw
+constexpr uint64_t kNormSpan = OPT_NORM_UNITS * OPT_STRIDE;       // elements of a workgroup of k_grad_norm
+
+int log2_of(uint64_t power) { return __builtin_ctzll(power); }
+
+// Strides of a workgroup of k_adamw.
+uint32_t adamw_span(uint64_t total, bool eight) {
+    if (const char* e = tune_env("GCN_TUNE_ADAMW_UNITS")) return (uint32_t)atoi(e) * OPT_STRIDE;
+    return OPT_STRIDE;
+}
 
 size_t elem_size(int type) { return type == GCN_F32 ? 4 : 2; }
 
 bool aligned_to(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
-uint64_t units_of(uint64_t n, uint64_t unit) { return (n + unit - 1) / unit; }
+uint64_t units_of(uint64_t n, uint64_t span) { return (n + span - 1) / span; }
 
-// strides of a workgroup of k_grad_norm: enough workgroups to fill the chip, few enough partial sums for one workgroup to add
-int norm_units(uint64_t total) { return total <= (1ull << 24) ? 2 : total <= (1ull << 28) ? 16 : 64; }
+void put(OptTable* t, int field, int k, uint64_t value) {
+    const int e = field * t->cap + k;
+    t->lo[e] = (uint32_t)value;
+    const int shift = 16 * (e & 1);
+    t->hi[e >> 1] = (t->hi[e >> 1] & ~(0xFFFFu << shift)) | (uint32_t)(value >> 32 & 0xFFFFu) << shift;
+}
+
+// A table has 47 bits for an address.
+bool fits(const void* p) { return ((uintptr_t)p >> 47) == 0; }
 
 int check_numel(const char* who, int n, const long long* numel, uint64_t* total) {
     *total = 0;
@@ -76,37 +91,42 @@ int gcn_adamw_step(const gcn_adamw_desc* d, void* const* params, const void* con
         if (!aligned_to(params[k], pe) || !aligned_to(grads[k], pe) || !aligned_to(exp_avg[k], se) || !aligned_to(exp_avg_sq[k], se) ||
             (half && !aligned_to(masters[k], 4)))
             return fail(-1, "gcn_adamw_step: tensor %d is not aligned to its elements", k);
+        if (!fits(params[k]) || !fits(grads[k]) || !fits(exp_avg[k]) || !fits(exp_avg_sq[k]) || (half && !fits(masters[k])) ||
+            (eight && (!fits(exp_avg_exp[k]) || !fits(exp_avg_sq_exp[k]))))
+            return fail(-2, "gcn_adamw_step: tensor %d lies beyond the addresses that the kernel's table holds", k);
     }
     hipStream_t st = (hipStream_t)stream;
     const AdamwHyper h = hyper ? AdamwHyper{} : opt_hyper(d->lr, d->beta1, d->beta2, d->eps, d->weight_decay, d->step, d->seed);
-    OptTable t;
-    t.stride = 5 + (half ? 1 : 0) + (eight ? 2 : 0);
-    const int most = std::min(OPT_MAX_TENSORS, OPT_WORDS / t.stride);
+    OptTable t = {};
+    t.span = adamw_span(total, eight);
+    t.span_log2 = log2_of(t.span);
+    t.cap = OPT_ENTRIES / (5 + (half ? 1 : 0) + (eight ? 2 : 0));
     for (int k = 0; k < d->n;) {
         t.n = 0;
         t.ordinal = d->first_tensor + (uint32_t)k;
         uint64_t blocks = 0;
         // tensors keep their numbers: an empty one takes a place without workgroups
-        for (; k < d->n && t.n < most; ++k, ++t.n) {
-            const uint64_t more = units_of((uint64_t)numel[k], kAdamwUnits * OPT_STRIDE);
+        for (; k < d->n && t.n < t.cap; ++k, ++t.n) {
+            const uint64_t more = units_of((uint64_t)numel[k], t.span);
             if (blocks + more > 0x7fffffffull) {
                 if (t.n == 0) return fail(-2, "gcn_adamw_step: tensor %d is too large for one launch", k);
                 break;
             }
-            uint64_t* w = t.w + (size_t)t.n * t.stride;
             bool vec = aligned_to(params[k], 16) && aligned_to(grads[k], 16) && aligned_to(exp_avg[k], eight ? 8 : 16) && aligned_to(exp_avg_sq[k], eight ? 8 : 16);
             if (half) vec = vec && aligned_to(masters[k], 16);
-            w[0] = (uint64_t)numel[k] | (vec ? OPT_VEC : 0);
-            w[1] = (uint64_t)params[k]; w[2] = (uint64_t)grads[k]; w[3] = (uint64_t)exp_avg[k]; w[4] = (uint64_t)exp_avg_sq[k];
-            int at = 5;
-            if (half) w[at++] = (uint64_t)masters[k];
-            if (eight) { w[at++] = (uint64_t)exp_avg_exp[k]; w[at] = (uint64_t)exp_avg_sq_exp[k]; }
-            t.first[t.n] = (uint32_t)blocks;
+            put(&t, 0, t.n, (uint64_t)numel[k] | (vec ? OPT_VEC : 0));
+            put(&t, 1, t.n, (uint64_t)params[k]);
+            put(&t, 2, t.n, (uint64_t)grads[k]);
+            put(&t, 3, t.n, (uint64_t)exp_avg[k]);
+            put(&t, 4, t.n, (uint64_t)exp_avg_sq[k]);
+            int field = 5;
+            if (half) put(&t, field++, t.n, (uint64_t)masters[k]);
+            if (eight) { put(&t, field++, t.n, (uint64_t)exp_avg_exp[k]); put(&t, field, t.n, (uint64_t)exp_avg_sq_exp[k]); }
             blocks += more;
         }
         if (blocks == 0) continue;
         GCN_PROF_PRE("k_adamw");
-#define ADAMW_LAUNCH(P, M, E) k_adamw<kAdamwUnits, P, M, E><<<(uint32_t)blocks, OPT_THREADS, 0, st>>>(t, h, (const AdamwHyper*)hyper, grad_scale, clip_coef)
+#define ADAMW_LAUNCH(P, M, E) k_adamw<P, M, E><<<(uint32_t)blocks, OPT_THREADS, 0, st>>>(t, h, (const AdamwHyper*)hyper, grad_scale, clip_coef)
         if (d->param_type == GCN_F32) { if (eight) ADAMW_LAUNCH(float, false, true); else ADAMW_LAUNCH(float, false, false); }
         else if (d->param_type == GCN_BF16) { if (eight) ADAMW_LAUNCH(__bf16, true, true); else ADAMW_LAUNCH(__bf16, true, false); }
         else { if (eight) ADAMW_LAUNCH(_Float16, true, true); else ADAMW_LAUNCH(_Float16, true, false); }
@@ -119,8 +139,7 @@ int gcn_adamw_step(const gcn_adamw_desc* d, void* const* params, const void* con
 size_t gcn_grad_norm_ws_bytes(int n, const long long* numel) {
     uint64_t total = 0, blocks = 0;
     if (n < 0 || (n > 0 && !numel) || check_numel("gcn_grad_norm_ws_bytes", n, numel, &total)) return 0;
-    const int units = norm_units(total);
-    for (int k = 0; k < n; ++k) blocks += units_of((uint64_t)numel[k], (uint64_t)units * OPT_STRIDE);
+    for (int k = 0; k < n; ++k) blocks += units_of((uint64_t)numel[k], kNormSpan);
     return std::max<size_t>(blocks, 1) * sizeof(double);
 }
 
@@ -133,37 +152,35 @@ int gcn_grad_norm(int n, int type, const void* const* grads, const long long* nu
     if (int rc = check_numel("gcn_grad_norm", n, numel, &total)) return rc;
     for (int k = 0; k < n; ++k)
         if (numel[k] > 0 && (!grads[k] || !aligned_to(grads[k], elem_size(type)))) return fail(-1, "gcn_grad_norm: tensor %d has a null or misaligned pointer", k);
+    for (int k = 0; k < n; ++k)
+        if (numel[k] > 0 && !fits(grads[k])) return fail(-2, "gcn_grad_norm: tensor %d lies beyond the addresses that the kernel's table holds", k);
     if (!ws || !aligned_to(ws, 8) || ws_bytes < gcn_grad_norm_ws_bytes(n, numel)) return fail(-2, "gcn_grad_norm: workspace too small");
     hipStream_t st = (hipStream_t)stream;
-    const int units = norm_units(total);
     double* part = (double*)ws;
     uint64_t done = 0;
-    OptTable t;
-    t.stride = 2;
+    OptTable t = {};
+    t.span = (uint32_t)kNormSpan;
+    t.span_log2 = log2_of(kNormSpan);
+    t.cap = OPT_ENTRIES / 2;
     t.ordinal = 0;
     for (int k = 0; k < n;) {
         t.n = 0;
         uint64_t blocks = 0;
-        for (; k < n && t.n < OPT_MAX_TENSORS; ++k, ++t.n) {
-            const uint64_t more = units_of((uint64_t)numel[k], (uint64_t)units * OPT_STRIDE);
+        for (; k < n && t.n < t.cap; ++k, ++t.n) {
+            const uint64_t more = units_of((uint64_t)numel[k], kNormSpan);
             if (blocks + more > 0x7fffffffull) {
                 if (t.n == 0) return fail(-2, "gcn_grad_norm: tensor %d is too large for one launch", k);
                 break;
             }
-            t.w[2 * t.n] = (uint64_t)numel[k] | (aligned_to(grads[k], 16) ? OPT_VEC : 0);
-            t.w[2 * t.n + 1] = (uint64_t)grads[k];
-            t.first[t.n] = (uint32_t)blocks;
+            put(&t, 0, t.n, (uint64_t)numel[k] | (aligned_to(grads[k], 16) ? OPT_VEC : 0));
+            put(&t, 1, t.n, (uint64_t)grads[k]);
             blocks += more;
         }
         if (blocks == 0) continue;
         GCN_PROF_PRE("k_grad_norm");
-#define NORM_LAUNCH(U, P) k_grad_norm<U, P><<<(uint32_t)blocks, OPT_THREADS, 0, st>>>(t, part + done)
-#define NORM_LAUNCH_T(P) do { if (units == 2) NORM_LAUNCH(2, P); else if (units == 16) NORM_LAUNCH(16, P); else NORM_LAUNCH(64, P); } while (0)
-        if (type == GCN_F32) NORM_LAUNCH_T(float);
-        else if (type == GCN_BF16) NORM_LAUNCH_T(__bf16);
-        else NORM_LAUNCH_T(_Float16);
-#undef NORM_LAUNCH_T
-#undef NORM_LAUNCH
+        if (type == GCN_F32) k_grad_norm<float><<<(uint32_t)blocks, OPT_THREADS, 0, st>>>(t, part + done);
+        else if (type == GCN_BF16) k_grad_norm<__bf16><<<(uint32_t)blocks, OPT_THREADS, 0, st>>>(t, part + done);
+        else k_grad_norm<_Float16><<<(uint32_t)blocks, OPT_THREADS, 0, st>>>(t, part + done);
         GCN_CHECK_LAUNCH("k_grad_norm");
         done += blocks;
     }
