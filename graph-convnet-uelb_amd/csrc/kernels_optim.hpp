@@ -188,14 +188,14 @@ __device__ __forceinline__ uint32_t opt_exponent(uint32_t top) {
 }
 __device__ __forceinline__ float opt_pow2(uint32_t exponent_byte) { return __builtin_bit_cast(float, exponent_byte << 23); }
 
-// e4m3 code of |x| (x scaled to the block), rounded up if the 20 bits below the code's last one and the 16 random bits
-// carry.  Below 2^-6 the steps are 2^-9: adding 2^-6 moves the value into the binade that has these steps.
-__device__ __forceinline__ uint32_t opt_code(float scaled, uint32_t random16) {
+// e4m3 code of a value that is finite and scaled to its block (>= 0, < 512), rounded up if the 20 bits below the code's last
+// one and the 16 random bits (in place, shifted by 4) carry.  Below 2^-6 the steps are 2^-9: adding 2^-6 moves the value
+// into the binade that has these steps, which starts at code 0 instead of 8.
+__device__ __forceinline__ uint32_t opt_code(float scaled, uint32_t random) {
 #pragma clang fp contract(off)
     const bool small = scaled < 0.015625f;
     const float y = small ? scaled + 0.015625f : scaled;
-    const uint32_t c = ((__builtin_bit_cast(uint32_t, y) + (random16 << 4)) >> 20) - (small ? 968u : 960u);
-    return min(c, 126u);
+    return (__builtin_bit_cast(uint32_t, y) + random + (small ? 0u - (121u << 23) : 0u - (120u << 23))) >> 20;
 }
 
 template <typename P, bool MASTER, bool EIGHT>
@@ -229,7 +229,8 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adamw(OptTable t, AdamwHyper by
             uint32_t cm[2], cr[2];
             opt_load_codes((const uint8_t*)m_at, i, left, vec, cm);
             opt_load_codes((const uint8_t*)v_at, i, left, vec, cr);
-            const float sm = opt_pow2(left ? exp_m[i / OPT_BLOCK] : 0), sr = opt_pow2(left ? exp_v[i / OPT_BLOCK] : 0);
+            // a power of two times b1 is exact, and the product below rounds as b1 times the moment does
+            const float sm = opt_pow2(left ? exp_m[i / OPT_BLOCK] : 0) * h.b1, sr = opt_pow2(left ? exp_v[i / OPT_BLOCK] : 0);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], true);
@@ -246,21 +247,29 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adamw(OptTable t, AdamwHyper by
         for (int e = 0; e < OPT_PER_LANE; ++e) {
             const float ge = gi[e] * s;
             float v = EIGHT ? r[e] * r[e] : r[e];
-            m[e] = h.b1 * m[e] + h.omb1 * ge;
+            m[e] = (EIGHT ? m[e] : h.b1 * m[e]) + h.omb1 * ge;
             v = h.b2 * v + h.omb2 * (ge * ge);
             const float root = __builtin_sqrtf(v);
-            const float change = m[e] / (root * h.inv_sqrt_bc2 + h.eps);
+            const float below = root * h.inv_sqrt_bc2 + h.eps;
+            // 8 bits: the vector units are as busy as memory; the reciprocal (1 ulp, its argument is never near the ends of the
+            // range) saves 10 of 80 instructions an element
+            const float change = EIGHT ? m[e] * __builtin_amdgcn_rcpf(below) : m[e] / below;
             pi[e] = pi[e] * h.decay - h.step_size * change;
             r[e] = EIGHT ? root : v;
-            if constexpr (EIGHT) {
-                top_m = max(top_m, __builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu);
-                top_r = max(top_r, __builtin_bit_cast(uint32_t, root) & 0x7FFFFFFFu);
+        }
+        if constexpr (EIGHT) {
+#pragma unroll
+            for (int e = 0; e < OPT_PER_LANE; e += 2) {
+                top_m = max(max(top_m, __builtin_bit_cast(uint32_t, m[e]) << 1), __builtin_bit_cast(uint32_t, m[e + 1]) << 1);
+                top_r = max(max(top_r, __builtin_bit_cast(uint32_t, r[e])), __builtin_bit_cast(uint32_t, r[e + 1]));
             }
+            top_m >>= 1;
         }
         if constexpr (MASTER) opt_store(master, i, left, vec, pi);
         opt_store(p, i, left, vec, pi);
         if constexpr (EIGHT) {
-            if (max(top_m, top_r) >= 0x7F800000u) {              // a value that is not finite: the largest of the others
+            const bool bad = max(top_m, top_r) >= 0x7F800000u;   // a value that is not finite: the largest of the others
+            if (bad) {
                 top_m = top_r = 0;
 #pragma unroll
                 for (int e = 0; e < OPT_PER_LANE; ++e) {
@@ -272,17 +281,22 @@ __global__ __launch_bounds__(OPT_THREADS) void k_adamw(OptTable t, AdamwHyper by
             // elements behind the end are zeros (or not finite, by a scale that is not) and change no maximum
             const uint32_t em = opt_exponent(opt_max16(top_m)), er = opt_exponent(opt_max16(top_r));
             const float um = opt_pow2(254 - em), ur = opt_pow2(254 - er);
+            if (bad) {
+#pragma unroll
+                for (int e = 0; e < OPT_PER_LANE; ++e) {          // 448 times the block's scale: the largest code
+                    if ((__builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu) >= 0x7F800000u) m[e] = __builtin_copysignf(448.f * opt_pow2(em), m[e]);
+                    if ((__builtin_bit_cast(uint32_t, r[e]) & 0x7FFFFFFFu) >= 0x7F800000u) r[e] = 448.f * opt_pow2(er);
+                }
+            }
             uint32_t cm[2] = {0, 0}, cr[2] = {0, 0};
+            const uint32_t lane_key = key ^ (uint32_t)i ^ ((uint32_t)(i >> 32) * 0xC2B2AE35U);      // i is a multiple of 8
 #pragma unroll
             for (int e = 0; e < OPT_PER_LANE; ++e) {
-                const uint64_t place = i + e;
-                const uint32_t random = opt_mix(key ^ (uint32_t)place ^ ((uint32_t)(place >> 32) * 0xC2B2AE35U));
-                uint32_t a = opt_code(__builtin_fabsf(m[e]) * um, random & 0xFFFFu);
-                a |= m[e] < 0.f ? 128u : 0u;
-                uint32_t b = opt_code(r[e] * ur, random >> 16);
-                b = r[e] > 0.f ? max(b, 1u) : b;
-                cm[e >> 2] |= a << (8 * (e & 3));
-                cr[e >> 2] |= b << (8 * (e & 3));
+                const uint32_t random = opt_mix(lane_key ^ (uint32_t)e), at = 8 * (e & 3);
+                const uint32_t a = opt_code(__builtin_fabsf(m[e]) * um, random << 4 & 0xFFFF0u);
+                const uint32_t b = max(opt_code(r[e] * ur, random >> 12 & 0xFFFF0u), min(__builtin_bit_cast(uint32_t, r[e]), 1u));
+                cm[e >> 2] |= (a | (__builtin_bit_cast(uint32_t, m[e]) >> 24 & 128u)) << at;
+                cr[e >> 2] |= b << at;
             }
             opt_store_codes((uint8_t*)m_at, i, left, vec, cm);
             opt_store_codes((uint8_t*)v_at, i, left, vec, cr);
