@@ -85,12 +85,18 @@ __device__ __forceinline__ uint32_t opt_scan_step(uint32_t x) {
 }
 // The tensor that this workgroup works on and which of its units: a lane adds the units of a few tensors, a scan over the
 // wavefront places them (no table of first workgroups, whose room goes to more tensors).
+template <int MOST>
 __device__ __forceinline__ int opt_find(const OptTable& t, uint32_t* unit) {
     const int lane = threadIdx.x & 63, per = (t.n + 63) >> 6;
     const auto units = [&](int k) { return (uint32_t)(((opt_entry(t, 0, k) & ~OPT_VEC) + t.span - 1) >> t.span_log2); };
     uint32_t mine = 0;
-    for (int j = 0; j < per; ++j)
-        if (lane * per + j < t.n) mine += units(lane * per + j);
+#pragma unroll
+    for (int j = 0; j < (MOST + 63) / 64; ++j) {                    // all loads at once: places without a tensor read the first
+        const int k = lane * per + j;
+        const bool there = j < per && k < t.n;
+        const uint32_t u = units(there ? k : 0);
+        mine += there ? u : 0;
+    }
     uint32_t up_to = mine;                                          // sum over this lane and those before it
     up_to = opt_scan_step<0x111, 0xf>(up_to);
     up_to = opt_scan_step<0x112, 0xf>(up_to);
@@ -107,11 +113,11 @@ __device__ __forceinline__ int opt_find(const OptTable& t, uint32_t* unit) {
     return k;
 }
 
-// Eight elements at i: a 16-byte access for each four (16-bit types: eight) where `vec`, single ones otherwise and
-// where fewer than eight are left.
-template <typename T>
+// Eight elements at i: a 16-byte access for each four (16-bit types: eight) where `vec` (the tensor's addresses allow it) and
+// all eight exist, single ones otherwise.  FULL: both hold for the whole workgroup, and no branch stands between its loads.
+template <bool FULL, typename T>
 __device__ __forceinline__ void opt_load(const T* __restrict__ p, uint64_t i, int left, bool vec, float* out) {
-    if (vec && left >= OPT_PER_LANE) {
+    if (FULL || (vec && left >= OPT_PER_LANE)) {
         if constexpr (sizeof(T) == 4) {
             const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p + i), b = *reinterpret_cast<const f32x4_t*>(p + i + 4);
 #pragma unroll
@@ -127,9 +133,9 @@ __device__ __forceinline__ void opt_load(const T* __restrict__ p, uint64_t i, in
         for (int k = 0; k < OPT_PER_LANE; ++k) out[k] = k < left ? (float)p[i + k] : 0.f;
     }
 }
-template <typename T>
+template <bool FULL, typename T>
 __device__ __forceinline__ void opt_store(T* __restrict__ p, uint64_t i, int left, bool vec, const float* in) {
-    if (vec && left >= OPT_PER_LANE) {
+    if (FULL || (vec && left >= OPT_PER_LANE)) {
         if constexpr (sizeof(T) == 4) {
             f32x4_t a, b;
 #pragma unroll
@@ -149,8 +155,9 @@ __device__ __forceinline__ void opt_store(T* __restrict__ p, uint64_t i, int lef
             if (k < left) p[i + k] = (T)in[k];
     }
 }
+template <bool FULL>
 __device__ __forceinline__ void opt_load_codes(const uint8_t* __restrict__ p, uint64_t i, int left, bool vec, uint32_t* out) {
-    if (vec && left >= OPT_PER_LANE) {
+    if (FULL || (vec && left >= OPT_PER_LANE)) {
         const uint2 a = *reinterpret_cast<const uint2*>(p + i);
         out[0] = a.x; out[1] = a.y;
     } else {
@@ -160,8 +167,9 @@ __device__ __forceinline__ void opt_load_codes(const uint8_t* __restrict__ p, ui
             if (k < left) out[k >> 2] |= (uint32_t)p[i + k] << (8 * (k & 3));
     }
 }
+template <bool FULL>
 __device__ __forceinline__ void opt_store_codes(uint8_t* __restrict__ p, uint64_t i, int left, bool vec, const uint32_t* in) {
-    if (vec && left >= OPT_PER_LANE) {
+    if (FULL || (vec && left >= OPT_PER_LANE)) {
         *reinterpret_cast<uint2*>(p + i) = make_uint2(in[0], in[1]);
     } else {
 #pragma unroll
@@ -198,116 +206,132 @@ __device__ __forceinline__ uint32_t opt_code(float scaled, uint32_t random) {
     return (__builtin_bit_cast(uint32_t, y) + random + (small ? 0u - (121u << 23) : 0u - (120u << 23))) >> 20;
 }
 
+template <typename P>
+struct AdamwTensor {
+    P* p;
+    const P* g;
+    void *m, *v;
+    float* master;
+    uint8_t *exp_m, *exp_v;
+};
+// Eight elements of every lane, from i on; `left` of them exist (FULL: all).
+template <bool FULL, typename P, bool MASTER, bool EIGHT>
+__device__ __forceinline__ void adamw_elements(const AdamwTensor<P>& w, uint64_t i, int left, bool vec, const AdamwHyper& h, float s, uint32_t key) {
+#pragma clang fp contract(off)
+    float gi[OPT_PER_LANE], pi[OPT_PER_LANE], m[OPT_PER_LANE], r[OPT_PER_LANE];
+    opt_load<FULL>(w.g, i, left, vec, gi);
+    if constexpr (MASTER) opt_load<FULL>(w.master, i, left, vec, pi);
+    else opt_load<FULL>(w.p, i, left, vec, pi);
+    if constexpr (EIGHT) {
+        uint32_t cm[2], cr[2];
+        opt_load_codes<FULL>((const uint8_t*)w.m, i, left, vec, cm);
+        opt_load_codes<FULL>((const uint8_t*)w.v, i, left, vec, cr);
+        // a power of two times b1 is exact, and the product below rounds as b1 times the moment does
+        const float sm = opt_pow2(FULL || left ? w.exp_m[i / OPT_BLOCK] : 0) * h.b1, sr = opt_pow2(FULL || left ? w.exp_v[i / OPT_BLOCK] : 0);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], true);
+            const auto c = __builtin_amdgcn_cvt_pk_f32_fp8(cr[q], false), d = __builtin_amdgcn_cvt_pk_f32_fp8(cr[q], true);
+            m[4 * q] = a[0] * sm; m[4 * q + 1] = a[1] * sm; m[4 * q + 2] = b[0] * sm; m[4 * q + 3] = b[1] * sm;
+            r[4 * q] = c[0] * sr; r[4 * q + 1] = c[1] * sr; r[4 * q + 2] = d[0] * sr; r[4 * q + 3] = d[1] * sr;
+        }
+    } else {
+        opt_load<FULL>((const float*)w.m, i, left, vec, m);
+        opt_load<FULL>((const float*)w.v, i, left, vec, r);
+    }
+    uint32_t top_m = 0, top_r = 0;
+#pragma unroll
+    for (int e = 0; e < OPT_PER_LANE; ++e) {
+        const float ge = gi[e] * s;
+        float v = EIGHT ? r[e] * r[e] : r[e];
+        m[e] = (EIGHT ? m[e] : h.b1 * m[e]) + h.omb1 * ge;
+        v = h.b2 * v + h.omb2 * (ge * ge);
+        const float root = __builtin_sqrtf(v);
+        const float below = root * h.inv_sqrt_bc2 + h.eps;
+        // 8 bits: the vector units are as busy as memory; the reciprocal (1 ulp, its argument is never near the ends of the
+        // range) saves 10 of 80 instructions an element
+        const float change = EIGHT ? m[e] * __builtin_amdgcn_rcpf(below) : m[e] / below;
+        pi[e] = pi[e] * h.decay - h.step_size * change;
+        r[e] = EIGHT ? root : v;
+    }
+    if constexpr (EIGHT) {
+#pragma unroll
+        for (int e = 0; e < OPT_PER_LANE; e += 2) {
+            top_m = max(max(top_m, __builtin_bit_cast(uint32_t, m[e]) << 1), __builtin_bit_cast(uint32_t, m[e + 1]) << 1);
+            top_r = max(max(top_r, __builtin_bit_cast(uint32_t, r[e])), __builtin_bit_cast(uint32_t, r[e + 1]));
+        }
+        top_m >>= 1;
+    }
+    if constexpr (MASTER) opt_store<FULL>(w.master, i, left, vec, pi);
+    opt_store<FULL>(w.p, i, left, vec, pi);
+    if constexpr (EIGHT) {
+        const bool bad = max(top_m, top_r) >= 0x7F800000u;   // a value that is not finite: the largest of the others
+        if (bad) {
+            top_m = top_r = 0;
+#pragma unroll
+            for (int e = 0; e < OPT_PER_LANE; ++e) {
+                const uint32_t bm = __builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu, br = __builtin_bit_cast(uint32_t, r[e]) & 0x7FFFFFFFu;
+                top_m = max(top_m, bm < 0x7F800000u ? bm : 0u);
+                top_r = max(top_r, br < 0x7F800000u ? br : 0u);
+            }
+        }
+        // elements behind the end are zeros (or not finite, by a scale that is not) and change no maximum
+        const uint32_t em = opt_exponent(opt_max16(top_m)), er = opt_exponent(opt_max16(top_r));
+        const float um = opt_pow2(254 - em), ur = opt_pow2(254 - er);
+        if (bad) {
+#pragma unroll
+            for (int e = 0; e < OPT_PER_LANE; ++e) {          // 448 times the block's scale: the largest code
+                if ((__builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu) >= 0x7F800000u) m[e] = __builtin_copysignf(448.f * opt_pow2(em), m[e]);
+                if ((__builtin_bit_cast(uint32_t, r[e]) & 0x7FFFFFFFu) >= 0x7F800000u) r[e] = 448.f * opt_pow2(er);
+            }
+        }
+        uint32_t cm[2] = {0, 0}, cr[2] = {0, 0};
+        const uint32_t lane_key = key ^ (uint32_t)i ^ ((uint32_t)(i >> 32) * 0xC2B2AE35U);      // i is a multiple of 8
+#pragma unroll
+        for (int e = 0; e < OPT_PER_LANE; ++e) {
+            const uint32_t random = opt_mix(lane_key ^ (uint32_t)e), at = 8 * (e & 3);
+            const uint32_t a = opt_code(__builtin_fabsf(m[e]) * um, random << 4 & 0xFFFF0u);
+            const uint32_t b = max(opt_code(r[e] * ur, random >> 12 & 0xFFFF0u), min(__builtin_bit_cast(uint32_t, r[e]), 1u));
+            cm[e >> 2] |= (a | (__builtin_bit_cast(uint32_t, m[e]) >> 24 & 128u)) << at;
+            cr[e >> 2] |= b << at;
+        }
+        opt_store_codes<FULL>((uint8_t*)w.m, i, left, vec, cm);
+        opt_store_codes<FULL>((uint8_t*)w.v, i, left, vec, cr);
+        if ((threadIdx.x & 15) == 0 && (FULL || left > 0)) {
+            w.exp_m[i / OPT_BLOCK] = (uint8_t)em;
+            w.exp_v[i / OPT_BLOCK] = (uint8_t)er;
+        }
+    } else {
+        opt_store<FULL>((float*)w.m, i, left, vec, m);
+        opt_store<FULL>((float*)w.v, i, left, vec, r);
+    }
+}
+
 template <typename P, bool MASTER, bool EIGHT>
 __global__ __launch_bounds__(OPT_THREADS) void k_adamw(OptTable t, AdamwHyper by_value, const AdamwHyper* __restrict__ in_memory,
                                                        const float* __restrict__ grad_scale, const float* __restrict__ clip) {
-#pragma clang fp contract(off)
     uint32_t unit;
-    const int k = opt_find(t, &unit);
+    const int k = opt_find<OPT_ENTRIES / 5>(t, &unit);
     const uint64_t size = opt_entry(t, 0, k), n = size & ~OPT_VEC;
     const bool vec = (size & OPT_VEC) != 0;
-    P* p = (P*)opt_entry(t, 1, k);
-    const P* g = (const P*)opt_entry(t, 2, k);
-    void *m_at = (void*)opt_entry(t, 3, k), *v_at = (void*)opt_entry(t, 4, k);
-    float* master = MASTER ? (float*)opt_entry(t, 5, k) : nullptr;
-    uint8_t *exp_m = nullptr, *exp_v = nullptr;
-    if constexpr (EIGHT) { exp_m = (uint8_t*)opt_entry(t, MASTER ? 6 : 5, k); exp_v = (uint8_t*)opt_entry(t, MASTER ? 7 : 6, k); }
+    AdamwTensor<P> w = {(P*)opt_entry(t, 1, k), (const P*)opt_entry(t, 2, k), (void*)opt_entry(t, 3, k), (void*)opt_entry(t, 4, k),
+                        MASTER ? (float*)opt_entry(t, 5, k) : nullptr, EIGHT ? (uint8_t*)opt_entry(t, MASTER ? 6 : 5, k) : nullptr,
+                        EIGHT ? (uint8_t*)opt_entry(t, MASTER ? 7 : 6, k) : nullptr};
     const AdamwHyper h = in_memory ? *in_memory : by_value;
     const float s = (grad_scale ? *grad_scale : 1.f) * (clip ? *clip : 1.f);
     const uint32_t key = EIGHT ? opt_mix(h.key ^ ((t.ordinal + (uint32_t)k) * 0x85EBCA6BU)) : 0;
-    const uint64_t start = (uint64_t)unit << t.span_log2;
-    for (uint32_t at = 0; at < t.span; at += OPT_STRIDE) {
-        const uint64_t i = start + at + threadIdx.x * OPT_PER_LANE;
+    uint64_t i = ((uint64_t)unit << t.span_log2) + threadIdx.x * OPT_PER_LANE;
+    const uint64_t end = min(n, (uint64_t)(unit + 1) << t.span_log2);
+    if (vec && end == (uint64_t)(unit + 1) << t.span_log2) {
+        for (; i < end; i += OPT_STRIDE) adamw_elements<true, P, MASTER, EIGHT>(w, i, OPT_PER_LANE, true, h, s, key);
+        return;
+    }
+    // the last workgroup of a tensor, and tensors at odd addresses
+    for (uint32_t at = 0; at < t.span; at += OPT_STRIDE, i += OPT_STRIDE) {
         const int left = i < n ? (int)min(n - i, (uint64_t)OPT_PER_LANE) : 0;
         // a wavefront without elements leaves; one with some keeps all its lanes for the blocks' maxima
         if (__ballot(left > 0) == 0) break;
-        float gi[OPT_PER_LANE], pi[OPT_PER_LANE], m[OPT_PER_LANE], r[OPT_PER_LANE];
-        opt_load(g, i, left, vec, gi);
-        if constexpr (MASTER) opt_load(master, i, left, vec, pi);
-        else opt_load(p, i, left, vec, pi);
-        if constexpr (EIGHT) {
-            uint32_t cm[2], cr[2];
-            opt_load_codes((const uint8_t*)m_at, i, left, vec, cm);
-            opt_load_codes((const uint8_t*)v_at, i, left, vec, cr);
-            // a power of two times b1 is exact, and the product below rounds as b1 times the moment does
-            const float sm = opt_pow2(left ? exp_m[i / OPT_BLOCK] : 0) * h.b1, sr = opt_pow2(left ? exp_v[i / OPT_BLOCK] : 0);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], true);
-                const auto c = __builtin_amdgcn_cvt_pk_f32_fp8(cr[q], false), d = __builtin_amdgcn_cvt_pk_f32_fp8(cr[q], true);
-                m[4 * q] = a[0] * sm; m[4 * q + 1] = a[1] * sm; m[4 * q + 2] = b[0] * sm; m[4 * q + 3] = b[1] * sm;
-                r[4 * q] = c[0] * sr; r[4 * q + 1] = c[1] * sr; r[4 * q + 2] = d[0] * sr; r[4 * q + 3] = d[1] * sr;
-            }
-        } else {
-            opt_load((const float*)m_at, i, left, vec, m);
-            opt_load((const float*)v_at, i, left, vec, r);
-        }
-        uint32_t top_m = 0, top_r = 0;
-#pragma unroll
-        for (int e = 0; e < OPT_PER_LANE; ++e) {
-            const float ge = gi[e] * s;
-            float v = EIGHT ? r[e] * r[e] : r[e];
-            m[e] = (EIGHT ? m[e] : h.b1 * m[e]) + h.omb1 * ge;
-            v = h.b2 * v + h.omb2 * (ge * ge);
-            const float root = __builtin_sqrtf(v);
-            const float below = root * h.inv_sqrt_bc2 + h.eps;
-            // 8 bits: the vector units are as busy as memory; the reciprocal (1 ulp, its argument is never near the ends of the
-            // range) saves 10 of 80 instructions an element
-            const float change = EIGHT ? m[e] * __builtin_amdgcn_rcpf(below) : m[e] / below;
-            pi[e] = pi[e] * h.decay - h.step_size * change;
-            r[e] = EIGHT ? root : v;
-        }
-        if constexpr (EIGHT) {
-#pragma unroll
-            for (int e = 0; e < OPT_PER_LANE; e += 2) {
-                top_m = max(max(top_m, __builtin_bit_cast(uint32_t, m[e]) << 1), __builtin_bit_cast(uint32_t, m[e + 1]) << 1);
-                top_r = max(max(top_r, __builtin_bit_cast(uint32_t, r[e])), __builtin_bit_cast(uint32_t, r[e + 1]));
-            }
-            top_m >>= 1;
-        }
-        if constexpr (MASTER) opt_store(master, i, left, vec, pi);
-        opt_store(p, i, left, vec, pi);
-        if constexpr (EIGHT) {
-            const bool bad = max(top_m, top_r) >= 0x7F800000u;   // a value that is not finite: the largest of the others
-            if (bad) {
-                top_m = top_r = 0;
-#pragma unroll
-                for (int e = 0; e < OPT_PER_LANE; ++e) {
-                    const uint32_t bm = __builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu, br = __builtin_bit_cast(uint32_t, r[e]) & 0x7FFFFFFFu;
-                    top_m = max(top_m, bm < 0x7F800000u ? bm : 0u);
-                    top_r = max(top_r, br < 0x7F800000u ? br : 0u);
-                }
-            }
-            // elements behind the end are zeros (or not finite, by a scale that is not) and change no maximum
-            const uint32_t em = opt_exponent(opt_max16(top_m)), er = opt_exponent(opt_max16(top_r));
-            const float um = opt_pow2(254 - em), ur = opt_pow2(254 - er);
-            if (bad) {
-#pragma unroll
-                for (int e = 0; e < OPT_PER_LANE; ++e) {          // 448 times the block's scale: the largest code
-                    if ((__builtin_bit_cast(uint32_t, m[e]) & 0x7FFFFFFFu) >= 0x7F800000u) m[e] = __builtin_copysignf(448.f * opt_pow2(em), m[e]);
-                    if ((__builtin_bit_cast(uint32_t, r[e]) & 0x7FFFFFFFu) >= 0x7F800000u) r[e] = 448.f * opt_pow2(er);
-                }
-            }
-            uint32_t cm[2] = {0, 0}, cr[2] = {0, 0};
-            const uint32_t lane_key = key ^ (uint32_t)i ^ ((uint32_t)(i >> 32) * 0xC2B2AE35U);      // i is a multiple of 8
-#pragma unroll
-            for (int e = 0; e < OPT_PER_LANE; ++e) {
-                const uint32_t random = opt_mix(lane_key ^ (uint32_t)e), at = 8 * (e & 3);
-                const uint32_t a = opt_code(__builtin_fabsf(m[e]) * um, random << 4 & 0xFFFF0u);
-                const uint32_t b = max(opt_code(r[e] * ur, random >> 12 & 0xFFFF0u), min(__builtin_bit_cast(uint32_t, r[e]), 1u));
-                cm[e >> 2] |= (a | (__builtin_bit_cast(uint32_t, m[e]) >> 24 & 128u)) << at;
-                cr[e >> 2] |= b << at;
-            }
-            opt_store_codes((uint8_t*)m_at, i, left, vec, cm);
-            opt_store_codes((uint8_t*)v_at, i, left, vec, cr);
-            if ((threadIdx.x & 15) == 0 && left > 0) {
-                exp_m[i / OPT_BLOCK] = (uint8_t)em;
-                exp_v[i / OPT_BLOCK] = (uint8_t)er;
-            }
-        } else {
-            opt_store((float*)m_at, i, left, vec, m);
-            opt_store((float*)v_at, i, left, vec, r);
-        }
+        adamw_elements<false, P, MASTER, EIGHT>(w, i, left, vec, h, s, key);
     }
 }
 
@@ -327,17 +351,21 @@ template <typename P>
 __global__ __launch_bounds__(OPT_THREADS) void k_grad_norm(OptTable t, double* __restrict__ part) {
     __shared__ double wave_sum[OPT_THREADS / 64];
     uint32_t unit;
-    const int k = opt_find(t, &unit);
+    const int k = opt_find<OPT_ENTRIES / 2>(t, &unit);
     const uint64_t size = opt_entry(t, 0, k), n = size & ~OPT_VEC;
-    const bool vec = (size & OPT_VEC) != 0;
     const P* g = (const P*)opt_entry(t, 1, k);
     const uint64_t start = (uint64_t)unit * (OPT_NORM_UNITS * OPT_STRIDE) + threadIdx.x * OPT_PER_LANE;
     double sum = 0.0;
     float x[OPT_NORM_UNITS][OPT_PER_LANE];
+    if ((size & OPT_VEC) && (uint64_t)(unit + 1) * (OPT_NORM_UNITS * OPT_STRIDE) <= n) {
 #pragma unroll
-    for (int u = 0; u < OPT_NORM_UNITS; ++u) {
-        const uint64_t i = start + u * OPT_STRIDE;
-        opt_load(g, i, i < n ? (int)min(n - i, (uint64_t)OPT_PER_LANE) : 0, vec, x[u]);
+        for (int u = 0; u < OPT_NORM_UNITS; ++u) opt_load<true>(g, start + u * OPT_STRIDE, OPT_PER_LANE, true, x[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < OPT_NORM_UNITS; ++u) {
+            const uint64_t i = start + u * OPT_STRIDE;
+            opt_load<false>(g, i, i < n ? (int)min(n - i, (uint64_t)OPT_PER_LANE) : 0, (size & OPT_VEC) != 0, x[u]);
+        }
     }
 #pragma unroll
     for (int u = 0; u < OPT_NORM_UNITS; ++u)
