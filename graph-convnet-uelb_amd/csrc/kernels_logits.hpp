@@ -24,6 +24,8 @@
 #define LGT_STRIDE (LGT_THREADS * LGT_PER_LANE)
 #define LGT_SEEN 0x80000000u                   // a count's flag: the token stands in the prompt
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
 struct LogitsArgs {
     const void* x;                 // logits
     void* y;                       // forward: result; backward: gradient of the logits (may be null)
@@ -66,26 +68,53 @@ __device__ __forceinline__ void lgt_count_one(long long id, long long l, long lo
         else atomicOr(&cnt[at], LGT_SEEN);
     }
 }
-template <typename ID>
-__device__ __forceinline__ void lgt_count_ids(const ID* __restrict__ ids, long long len, long long prompt, int v0, int n, uint32_t* cnt) {
-    constexpr int W = 16 / sizeof(ID);
+// A lane's first 16 bytes of row r's history, requested before anything else: loads return in order, so that they can be
+// counted while the logits are on the way.
+__device__ __forceinline__ u32x4_t lgt_first_ids(const LogitsArgs& a, int r) {
+    u32x4_t ids = {0, 0, 0, 0};
+    const int w = a.history_wide ? 2 : 4;
+    if ((long long)(threadIdx.x + 1) * w <= a.history_len)
+        ids = lgt_vec<uint32_t, 4>(static_cast<const uint32_t*>(a.history) + ((long long)r * a.history_len + threadIdx.x * w) * (a.history_wide ? 2 : 1));
+    return ids;
+}
+template <bool LONG, typename ID>
+__device__ __forceinline__ void lgt_count_ids(const ID* __restrict__ ids, u32x4_t first, long long len, long long prompt, int v0, int n, uint32_t* cnt) {
+    constexpr int W = 16 / sizeof(ID), STEP = LGT_THREADS * W, DEEP = 8;
     long long l = (long long)threadIdx.x * W;
-    for (; l + W <= len; l += LGT_THREADS * W) {
+    if (l + W <= len) {
+        const LgtVec<ID, W> some = __builtin_bit_cast(LgtVec<ID, W>, first);
+#pragma unroll
+        for (int k = 0; k < W; ++k) lgt_count_one(some[k], l + k, prompt, v0, n, cnt);
+        l += STEP;
+    }
+    if constexpr (LONG) {
+        for (; l + (DEEP - 1) * STEP + W <= len; l += DEEP * STEP) {
+            LgtVec<ID, W> some[DEEP];
+#pragma unroll
+            for (int j = 0; j < DEEP; ++j) some[j] = lgt_vec<ID, W>(ids + l + j * STEP);
+#pragma unroll
+            for (int j = 0; j < DEEP; ++j)
+#pragma unroll
+                for (int k = 0; k < W; ++k) lgt_count_one(some[j][k], l + j * STEP + k, prompt, v0, n, cnt);
+        }
+    }
+    for (; l + W <= len; l += STEP) {
         const LgtVec<ID, W> some = lgt_vec<ID, W>(ids + l);
 #pragma unroll
         for (int k = 0; k < W; ++k) lgt_count_one(some[k], l + k, prompt, v0, n, cnt);
     }
     for (; l < len; ++l) lgt_count_one(ids[l], l, prompt, v0, n, cnt);       // the one lane whose group is cut off
 }
-__device__ __forceinline__ void lgt_count(const LogitsArgs& a, int o, int v0, int n, uint32_t* cnt) {
+template <bool LONG>
+__device__ __forceinline__ void lgt_count(const LogitsArgs& a, int o, u32x4_t first, int v0, int n, uint32_t* cnt) {
     for (int k = threadIdx.x * 4; k < n; k += LGT_THREADS * 4) *reinterpret_cast<uint4*>(cnt + k) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     const int r = o % a.history_rows;
     long long len = a.lens ? lgt_int(a.lens, a.lens_wide, r) : a.history_len;
     len = len < a.history_len ? len : a.history_len;
     const long long prompt = a.prompts ? lgt_int(a.prompts, a.lens_wide, r) : 0, base = (long long)r * a.history_len;
-    if (a.history_wide) lgt_count_ids(static_cast<const long long*>(a.history) + base, len, prompt, v0, n, cnt);
-    else lgt_count_ids(static_cast<const int*>(a.history) + base, len, prompt, v0, n, cnt);
+    if (a.history_wide) lgt_count_ids<LONG>(static_cast<const long long*>(a.history) + base, first, len, prompt, v0, n, cnt);
+    else lgt_count_ids<LONG>(static_cast<const int*>(a.history) + base, first, len, prompt, v0, n, cnt);
     __syncthreads();
 }
 
@@ -139,7 +168,9 @@ __device__ __forceinline__ void lgt_store(T* p, long long e, int left, const flo
 }
 
 // ---------------------------------------------------------------------------------------------- token logits (inner = 1)
-template <typename T, int ITER>
+// LONG: histories of 8192 entries and more are read eight loads at a time (16 rows of 50021 with 32768 entries of int64: 15.5 -> 9 us,
+// most of it the load-by-load walk); the code for that costs shorter ones 12 to 15 %.
+template <typename T, int ITER, bool LONG>
 __global__ __launch_bounds__(LGT_THREADS) void k_logits(LogitsArgs a) {
     extern __shared__ __align__(16) uint32_t cnt[];
     const int o = blockIdx.x / a.chunks, v0 = (blockIdx.x % a.chunks) * (ITER * LGT_STRIDE), n = min(ITER * LGT_STRIDE, a.vocab - v0);
@@ -147,6 +178,8 @@ __global__ __launch_bounds__(LGT_THREADS) void k_logits(LogitsArgs a) {
     T* y = static_cast<T*>(a.y) + (long long)o * a.y_stride + v0;
     const int mask_row = a.mask_type ? o % a.mask_rows : 0;
     const float* bias = a.bias ? a.bias + (long long)(o % a.bias_rows) * a.vocab + v0 : nullptr;
+    u32x4_t ids = {0, 0, 0, 0};
+    if (a.history) ids = lgt_first_ids(a, o % a.history_rows);
     LgtVec<T, LGT_PER_LANE> raw[ITER];
     uint32_t on[ITER];
 #pragma unroll
@@ -158,7 +191,7 @@ __global__ __launch_bounds__(LGT_THREADS) void k_logits(LogitsArgs a) {
     const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
     const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
     const float pres = lgt_param(a.pres, a.pres_rows, a.pres_value, o), freq = lgt_param(a.freq, a.freq_rows, a.freq_value, o);
-    if (a.history) lgt_count(a, o, v0, n, cnt);
+    if (a.history) lgt_count<LONG>(a, o, ids, v0, n, cnt);
 #pragma unroll
     for (int t = 0; t < ITER; ++t) {
         const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE, left = n - e;
@@ -191,30 +224,92 @@ __global__ __launch_bounds__(LGT_THREADS) void k_logits(LogitsArgs a) {
 }
 
 // Rows r, r + R, ... (R = bias_rows) of one part, one after the other: the gradient of the logits row by row, that of the bias
-// in registers.
+// in registers.  The slope needs to know whether a token was seen, not how often: one bit per entry in LDS, so that three rows'
+// bits fit and a row takes one barrier: while a row is worked on, the next one's gradient, mask and history are on the way, and
+// the bits of the one after it are cleared.
+template <typename T>
+struct LgtRow {
+    int o;
+    float inv_tau, rho;
+    long long len;
+    u32x4_t ids;                                 // the lane's first 16 bytes of the history
+};
+template <typename T, int ITER>
+__device__ __forceinline__ void lgt_fetch(const LogitsArgs& a, int o, int v0, int n, LgtRow<T>* row, LgtVec<T, LGT_PER_LANE> (&raw)[ITER], uint32_t (&on)[ITER]) {
+    row->o = o;
+    row->len = 0;
+    if (a.history) {
+        const int r = o % a.history_rows;
+        row->ids = lgt_first_ids(a, r);
+        const long long len = a.lens ? lgt_int(a.lens, a.lens_wide, r) : a.history_len;
+        row->len = len < a.history_len ? len : a.history_len;
+    }
+    const int mask_row = a.mask_type ? o % a.mask_rows : 0;
+    const T* dy = static_cast<const T*>(a.dy) + (long long)o * a.y_stride + v0;
+#pragma unroll
+    for (int t = 0; t < ITER; ++t) {
+        const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE;
+        raw[t] = lgt_load(dy, e, n - e);
+        on[t] = lgt_on8(a, mask_row, v0 + e, n - e);
+    }
+    row->rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o);
+    row->inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
+}
+__device__ __forceinline__ void lgt_see(long long id, int v0, int n, uint32_t* bits) {
+    const unsigned long long at = (unsigned long long)(id - v0);
+    if (at < (unsigned long long)n) atomicOr(&bits[at >> 5], 1u << (at & 31));
+}
+// The bits of a fetched row's history.
+template <typename T>
+__device__ __forceinline__ void lgt_see_row(const LogitsArgs& a, const LgtRow<T>& row, int v0, int n, uint32_t* bits) {
+    const int w = a.history_wide ? 2 : 4;
+    const long long base = (long long)(row.o % a.history_rows) * a.history_len;
+    long long l = (long long)threadIdx.x * w;
+    if (l + w <= row.len) {
+        if (a.history_wide) {
+            lgt_see((long long)(((unsigned long long)row.ids[1] << 32) | row.ids[0]), v0, n, bits);
+            lgt_see((long long)(((unsigned long long)row.ids[3] << 32) | row.ids[2]), v0, n, bits);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) lgt_see((int)row.ids[k], v0, n, bits);
+        }
+        l += LGT_THREADS * w;
+    }
+    for (; l < row.len; l += LGT_THREADS * w)
+        for (int k = 0; k < w && l + k < row.len; ++k) lgt_see(lgt_int(a.history, a.history_wide, base + l + k), v0, n, bits);
+}
+
 template <typename T, int ITER>
 __global__ __launch_bounds__(LGT_THREADS) void k_logits_bwd(LogitsArgs a) {
-    extern __shared__ __align__(16) uint32_t cnt[];
+    constexpr int WORDS = ITER * LGT_STRIDE / 32;
+    __shared__ uint32_t bits[3][WORDS];
     uint32_t at = blockIdx.x;
     const int v0 = (int)(at % a.chunks) * (ITER * LGT_STRIDE), n = min(ITER * LGT_STRIDE, a.vocab - v0);
     at /= a.chunks;
     const int r = (int)(at % a.bias_rows), part = (int)(at / a.bias_rows), many = a.rows / a.bias_rows;
     const int first = (int)((long long)many * part / a.splits), last = (int)((long long)many * (part + 1) / a.splits);
     float sum[ITER][LGT_PER_LANE] = {};
+    LgtRow<T> next;
+    LgtVec<T, LGT_PER_LANE> next_raw[ITER];
+    uint32_t next_on[ITER];
+    if (first < last) lgt_fetch<T, ITER>(a, r + first * a.bias_rows, v0, n, &next, next_raw, next_on);
+    for (int k = threadIdx.x; k < 2 * WORDS; k += LGT_THREADS) bits[k / WORDS][k % WORDS] = 0;
+    __syncthreads();
+    int buffer = 0;
     for (int q = first; q < last; ++q) {
-        const int o = r + q * a.bias_rows, mask_row = a.mask_type ? o % a.mask_rows : 0;
-        const T* dy = static_cast<const T*>(a.dy) + (long long)o * a.y_stride + v0;
+        const LgtRow<T> row = next;
         LgtVec<T, LGT_PER_LANE> raw[ITER];
         uint32_t on[ITER];
 #pragma unroll
-        for (int t = 0; t < ITER; ++t) {
-            const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE;
-            raw[t] = lgt_load(dy, e, n - e);
-            on[t] = lgt_on8(a, mask_row, v0 + e, n - e);
+        for (int t = 0; t < ITER; ++t) { raw[t] = next_raw[t]; on[t] = next_on[t]; }
+        if (q + 1 < last) lgt_fetch<T, ITER>(a, r + (q + 1) * a.bias_rows, v0, n, &next, next_raw, next_on);
+        const int clear = buffer == 0 ? 2 : buffer - 1;               // two rows on: last read before the previous barrier
+        if (a.history) {
+            lgt_see_row(a, row, v0, n, bits[buffer]);
+            __syncthreads();
+            for (int k = threadIdx.x; k < WORDS; k += LGT_THREADS) bits[clear][k] = 0;
         }
-        const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
-        const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
-        if (a.history) lgt_count(a, o, v0, n, cnt);
+        const float inv_rho = 1.f / row.rho;
 #pragma unroll
         for (int t = 0; t < ITER; ++t) {
             const int e = t * LGT_STRIDE + threadIdx.x * LGT_PER_LANE, left = n - e;
@@ -222,25 +317,23 @@ __global__ __launch_bounds__(LGT_THREADS) void k_logits_bwd(LogitsArgs a) {
             float g[LGT_PER_LANE];
 #pragma unroll
             for (int k = 0; k < LGT_PER_LANE; ++k) {
-                g[k] = (on[t] >> k) & 1 ? (float)raw[t][k] * inv_tau : 0.f;
+                g[k] = (on[t] >> k) & 1 ? (float)raw[t][k] * row.inv_tau : 0.f;
                 sum[t][k] += g[k];
             }
             if (!a.y) continue;
             if (a.history) {
-                uint32_t c[LGT_PER_LANE];
-                *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(cnt + e);
-                *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(cnt + e + 4);
-                if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
-                    const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + v0;
+                const uint32_t seen = reinterpret_cast<const uint8_t*>(bits[buffer])[e >> 3] & on[t];
+                if (seen) {
+                    const T* x = static_cast<const T*>(a.x) + (long long)row.o * a.x_stride + v0;
                     const LgtVec<T, LGT_PER_LANE> xs = lgt_load(x, e, left);
 #pragma unroll
                     for (int k = 0; k < LGT_PER_LANE; ++k)
-                        if (c[k] && ((on[t] >> k) & 1)) g[k] *= (float)xs[k] > 0.f ? inv_rho : rho;
+                        if ((seen >> k) & 1) g[k] *= (float)xs[k] > 0.f ? inv_rho : row.rho;
                 }
             }
-            lgt_store(static_cast<T*>(a.y) + (long long)o * a.y_stride + v0, e, left, g);
+            lgt_store(static_cast<T*>(a.y) + (long long)row.o * a.y_stride + v0, e, left, g);
         }
-        if (a.history) __syncthreads();          // the counts are cleared for the next row
+        buffer = buffer == 2 ? 0 : buffer + 1;
     }
     if (a.dbias) {
         float* out = a.dbias + ((long long)part * a.bias_rows + r) * a.vocab + v0;
@@ -267,7 +360,7 @@ __global__ __launch_bounds__(LGT_THREADS) void k_scores(LogitsArgs a) {
     const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
     const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
     const float pres = lgt_param(a.pres, a.pres_rows, a.pres_value, o), freq = lgt_param(a.freq, a.freq_rows, a.freq_value, o);
-    if (a.history) lgt_count(a, o, v0, n, cnt);
+    if (a.history) lgt_count<false>(a, o, lgt_first_ids(a, o % a.history_rows), v0, n, cnt);
     const float* bias = a.bias ? a.bias + (long long)(o % a.bias_rows) * a.vocab + v0 : nullptr;
     const int mask_row = a.mask_type ? o % a.mask_rows : 0;
     for (int v = threadIdx.x; v < n; v += LGT_THREADS) {
@@ -317,7 +410,7 @@ __global__ __launch_bounds__(LGT_THREADS) void k_scores_bwd(LogitsArgs a) {
         const int o = r + q * a.bias_rows, mask_row = a.mask_type ? o % a.mask_rows : 0;
         const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
         const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
-        if (a.history) lgt_count(a, o, v0, n, cnt);
+        if (a.history) lgt_count<false>(a, o, lgt_first_ids(a, o % a.history_rows), v0, n, cnt);
         for (int v = threadIdx.x; v < n; v += LGT_THREADS)
             cnt[v] = (a.history && cnt[v] ? LGT_SEEN : 0) | (lgt_on(a, mask_row, v0 + v) ? 0 : LGT_OFF);
         __syncthreads();
@@ -393,11 +486,23 @@ __global__ __launch_bounds__(LGT_THREADS) void k_scores_bias_grad(LogitsArgs a, 
     if (lane == 0) dbias[at] = sum;
 }
 
-// The parts' sums of the bias gradient, added in order.
+// The parts' sums of the bias gradient: 32 columns and 8 groups of parts per workgroup, each group added in order, then the
+// groups.
 __global__ __launch_bounds__(256) void k_logits_bias_sum(long long n, int splits, const float* __restrict__ part, float* __restrict__ dbias) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
+    __shared__ float group_sum[8][32];
+    const int column = threadIdx.x & 31, group = threadIdx.x >> 5;
+    const long long i = (long long)blockIdx.x * 32 + column;
+    const int first = (int)((long long)splits * group / 8), last = (int)((long long)splits * (group + 1) / 8);
     float sum = 0.f;
-    for (int p = 0; p < splits; ++p) sum += part[p * n + i];
-    dbias[i] = sum;
+    if (i < n) {
+#pragma unroll 8
+        for (int p = first; p < last; ++p) sum += part[p * n + i];
+    }
+    group_sum[group][column] = sum;
+    __syncthreads();
+    if (group == 0 && i < n) {
+#pragma unroll
+        for (int g = 1; g < 8; ++g) sum += group_sum[g][column];
+        dbias[i] = sum;
+    }
 }

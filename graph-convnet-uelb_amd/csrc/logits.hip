@@ -76,12 +76,23 @@ int launch_fwd(const LogitsArgs& a, hipStream_t st) {
     const uint32_t blocks = (uint32_t)a.rows * a.chunks;
     const size_t lds = lds_of(a, true, false);
     GCN_PROF_PRE(a.inner == 1 ? "k_logits" : "k_scores");
+    const bool wide = a.chunk == 2 * LGT_STRIDE, far = a.history && a.history_len >= 8192;
     if (a.inner > 1) k_scores<T><<<blocks, LGT_THREADS, lds, st>>>(a);
-    else if (a.chunk == LGT_STRIDE) k_logits<T, 1><<<blocks, LGT_THREADS, lds, st>>>(a);
-    else if (a.chunk == 2 * LGT_STRIDE) k_logits<T, 2><<<blocks, LGT_THREADS, lds, st>>>(a);
-    else k_logits<T, 4><<<blocks, LGT_THREADS, lds, st>>>(a);
+    else if (wide && far) k_logits<T, 2, true><<<blocks, LGT_THREADS, lds, st>>>(a);
+    else if (wide) k_logits<T, 2, false><<<blocks, LGT_THREADS, lds, st>>>(a);
+    else if (far) k_logits<T, 1, true><<<blocks, LGT_THREADS, lds, st>>>(a);
+    else k_logits<T, 1, false><<<blocks, LGT_THREADS, lds, st>>>(a);
     GCN_CHECK_LAUNCH("k_logits");
     return 0;
+}
+
+// The backward kernel's own range of a row.
+void set_bwd_chunk(LogitsArgs* a) {
+    if (a->inner != 1) return;
+    int it = 1;
+    if (const char* e = tune_env("GCN_TUNE_LOGITS_BWD_IT")) it = atoi(e);
+    a->chunk = LGT_STRIDE * it;
+    a->chunks = (a->vocab + a->chunk - 1) / a->chunk;
 }
 
 // Parts of the rows that share a bias row: about 1024 workgroups, but sums of the parts (written and read in fp32) of at most
@@ -89,7 +100,9 @@ int launch_fwd(const LogitsArgs& a, hipStream_t st) {
 int splits_of(const LogitsArgs& a, bool want_bias, int type) {
     const long long many = a.rows / a.bias_rows, per_part = (long long)a.chunks * a.bias_rows;
     if (!want_bias) return (int)many;
-    long long splits = std::min(many, (1024 + per_part - 1) / per_part);
+    long long target = 1024;
+    if (const char* e = tune_env("GCN_TUNE_LOGITS_WG")) target = atoi(e);
+    long long splits = std::min(many, (target + per_part - 1) / per_part);
     const long long data = (long long)a.rows * a.vocab * a.inner * (type == GCN_F32 ? 8 : 4), part = 8ll * a.bias_rows * a.vocab;
     return (int)std::max(1ll, std::min(splits, std::max(data, 32ll << 20) / 8 / part));
 }
@@ -106,8 +119,8 @@ int launch_bwd(LogitsArgs a, float* dbias, int splits, float* parts, hipStream_t
     if (a.y || by_tile) {
         GCN_PROF_PRE(a.inner == 1 ? "k_logits_bwd" : "k_scores_bwd");
         if (a.inner > 1) k_scores_bwd<T><<<blocks, LGT_THREADS, lds, st>>>(a);
-        else if (a.chunk == LGT_STRIDE) k_logits_bwd<T, 1><<<blocks, LGT_THREADS, lds, st>>>(a);
-        else k_logits_bwd<T, 2><<<blocks, LGT_THREADS, lds, st>>>(a);
+        else if (a.chunk == LGT_STRIDE) k_logits_bwd<T, 1><<<blocks, LGT_THREADS, 0, st>>>(a);
+        else k_logits_bwd<T, 2><<<blocks, LGT_THREADS, 0, st>>>(a);
         GCN_CHECK_LAUNCH("k_logits_bwd");
     }
     if (!dbias) return 0;
@@ -119,7 +132,7 @@ int launch_bwd(LogitsArgs a, float* dbias, int splits, float* parts, hipStream_t
         GCN_CHECK_LAUNCH("k_scores_bias_grad");
     } else if (splits > 1) {
         GCN_PROF_PRE("k_logits_bias_sum");
-        k_logits_bias_sum<<<(uint32_t)((n + 255) / 256), 256, 0, st>>>(n, splits, parts, dbias);
+        k_logits_bias_sum<<<(uint32_t)((n + 31) / 32), 256, 0, st>>>(n, splits, parts, dbias);
         GCN_CHECK_LAUNCH("k_logits_bias_sum");
     }
     return 0;
@@ -144,6 +157,7 @@ int gcn_logits_process(const gcn_logits_desc* d, const void* in, void* out, void
 size_t gcn_logits_bwd_ws_bytes(const gcn_logits_desc* d) {
     LogitsArgs a;
     if (fill_args(d, &a) || a.rows == 0 || !a.bias) return 0;
+    set_bwd_chunk(&a);
     const int splits = splits_of(a, true, d->type);
     return splits > 1 && tile_fits(a) ? (size_t)splits * a.bias_rows * a.vocab * sizeof(float) : 0;
 }
@@ -158,6 +172,7 @@ int gcn_logits_process_bwd(const gcn_logits_desc* d, const void* in, const void*
     const size_t need = dbias ? gcn_logits_bwd_ws_bytes(d) : 0;
     if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 3))) return fail(-2, "gcn_logits_process_bwd: workspace too small");
     a.x = in; a.y = din; a.dy = dout;
+    set_bwd_chunk(&a);
     if (!dbias) a.bias_rows = 1;
     // a repetition penalty of one changes no slope: the history is not needed
     if (!din || (!a.rep && a.rep_value == 1.f)) a.history = nullptr;
