@@ -89,9 +89,7 @@ int launch_fwd(const LogitsArgs& a, hipStream_t st) {
 // The backward kernel's own range of a row.
 void set_bwd_chunk(LogitsArgs* a) {
     if (a->inner != 1) return;
-    int it = 1;
-    if (const char* e = tune_env("GCN_TUNE_LOGITS_BWD_IT")) it = atoi(e);
-    a->chunk = LGT_STRIDE * it;
+    a->chunk = LGT_STRIDE;
     a->chunks = (a->vocab + a->chunk - 1) / a->chunk;
 }
 
@@ -99,10 +97,11 @@ void set_bwd_chunk(LogitsArgs* a) {
 // an eighth of the gradient's bytes where that is more than a launch's worth.
 int splits_of(const LogitsArgs& a, bool want_bias, int type) {
     const long long many = a.rows / a.bias_rows, per_part = (long long)a.chunks * a.bias_rows;
-    if (!want_bias) return (int)many;
+    if (!want_bias && a.inner > 1) return (int)many;
     long long target = 1024;
     if (const char* e = tune_env("GCN_TUNE_LOGITS_WG")) target = atoi(e);
     long long splits = std::min(many, (target + per_part - 1) / per_part);
+    if (!want_bias) return (int)splits;
     const long long data = (long long)a.rows * a.vocab * a.inner * (type == GCN_F32 ? 8 : 4), part = 8ll * a.bias_rows * a.vocab;
     return (int)std::max(1ll, std::min(splits, std::max(data, 32ll << 20) / 8 / part));
 }
@@ -119,8 +118,7 @@ int launch_bwd(LogitsArgs a, float* dbias, int splits, float* parts, hipStream_t
     if (a.y || by_tile) {
         GCN_PROF_PRE(a.inner == 1 ? "k_logits_bwd" : "k_scores_bwd");
         if (a.inner > 1) k_scores_bwd<T><<<blocks, LGT_THREADS, lds, st>>>(a);
-        else if (a.chunk == LGT_STRIDE) k_logits_bwd<T, 1><<<blocks, LGT_THREADS, 0, st>>>(a);
-        else k_logits_bwd<T, 2><<<blocks, LGT_THREADS, 0, st>>>(a);
+        else k_logits_bwd<T><<<blocks, LGT_THREADS, 0, st>>>(a);
         GCN_CHECK_LAUNCH("k_logits_bwd");
     }
     if (!dbias) return 0;
