@@ -328,8 +328,8 @@ __global__ __launch_bounds__(LGT_THREADS) void k_logits_bwd(LogitsArgs a) {
 
 // ---------------------------------------------------------------------------------------------- scores (inner > 1)
 // A workgroup's tile: `chunk` vocabulary entries with all their inner elements, which follow each other in memory.  What depends
-// on the entry alone stands in LDS: forward the sum of its additive terms, backward nothing, and two flags in the count.
-#define LGT_OFF 0x40000000u                    // replaces the count once it is used: the mask has the entry off
+// on the entry alone stands in LDS: the sum of its additive terms, and two flags in the count's place.
+#define LGT_OFF 0x40000000u                    // the mask has the entry off
 
 __device__ __forceinline__ int lgt_entry(int e, float inv_inner) { return (int)((e + 0.5f) * inv_inner); }    // e < 2^22: exact
 
@@ -338,10 +338,16 @@ __global__ __launch_bounds__(LGT_THREADS) void k_scores(LogitsArgs a) {
     extern __shared__ __align__(16) uint32_t cnt[];
     const int o = blockIdx.x / a.chunks, v0 = (blockIdx.x % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0);
     float* add = reinterpret_cast<float*>(cnt + ((a.chunk + 3) & ~3));
+    const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + (long long)v0 * a.inner;
+    T* y = static_cast<T*>(a.y) + (long long)o * a.y_stride + (long long)v0 * a.inner;
+    const int end = n * a.inner;
+    u32x4_t ids = {0, 0, 0, 0};
+    if (a.history) ids = lgt_first_ids(a, o % a.history_rows);
+    LgtVec<T, LGT_PER_LANE> raw = lgt_load(x, threadIdx.x * LGT_PER_LANE, end - (int)threadIdx.x * LGT_PER_LANE);
     const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
     const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
     const float pres = lgt_param(a.pres, a.pres_rows, a.pres_value, o), freq = lgt_param(a.freq, a.freq_rows, a.freq_value, o);
-    if (a.history) lgt_count<false>(a, o, lgt_first_ids(a, o % a.history_rows), v0, n, cnt);
+    if (a.history) lgt_count<false>(a, o, ids, v0, n, cnt);
     const float* bias = a.bias ? a.bias + (long long)(o % a.bias_rows) * a.vocab + v0 : nullptr;
     const int mask_row = a.mask_type ? o % a.mask_rows : 0;
     for (int v = threadIdx.x; v < n; v += LGT_THREADS) {
@@ -352,12 +358,9 @@ __global__ __launch_bounds__(LGT_THREADS) void k_scores(LogitsArgs a) {
         cnt[v] = (c ? LGT_SEEN : 0) | (lgt_on(a, mask_row, v0 + v) ? 0 : LGT_OFF);
     }
     __syncthreads();
-    const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + (long long)v0 * a.inner;
-    T* y = static_cast<T*>(a.y) + (long long)o * a.y_stride + (long long)v0 * a.inner;
-    const int end = n * a.inner;
     const float inv_inner = 1.f / (float)a.inner;
     for (int e = threadIdx.x * LGT_PER_LANE; e < end; e += LGT_STRIDE) {
-        const LgtVec<T, LGT_PER_LANE> raw = lgt_load(x, e, end - e);
+        if (e >= LGT_STRIDE) raw = lgt_load(x, e, end - e);
         float z[LGT_PER_LANE];
         int v = n == 1 ? 0 : lgt_entry(e, inv_inner), i = e - v * a.inner;
 #pragma unroll
@@ -372,12 +375,21 @@ __global__ __launch_bounds__(LGT_THREADS) void k_scores(LogitsArgs a) {
     }
 }
 
+#define LGT_SCORE_ROWS 8                       // rows of a turn
+#define LGT_SCORE_ENTRIES (LGT_STRIDE / 2)     // most entries of a tile
+
+// As k_logits_bwd: the histories of a turn's rows first, then their tiles one after the other, the next one on the way.  For the bias
+// the tile's gradient goes through LDS (two tiles in turn, one barrier a row): a group of lanes adds an entry's elements, and
+// keeps the sum over the rows in a register.
 template <typename T>
 __global__ __launch_bounds__(LGT_THREADS) void k_scores_bwd(LogitsArgs a) {
-    extern __shared__ __align__(16) uint32_t cnt[];
-    float* tile = reinterpret_cast<float*>(cnt + ((a.chunk + 3) & ~3));        // only with dbias: chunk * inner elements
+    __shared__ uint32_t seen[LGT_SCORE_ROWS * LGT_SCORE_ENTRIES / 32];
+    __shared__ float slope[LGT_SCORE_ROWS][2];
+    __shared__ int length[LGT_SCORE_ROWS];
+    extern __shared__ __align__(16) float tile[];             // with dbias: two of LGT_STRIDE elements; then a flag per (row, entry)
+    uint8_t* flag = reinterpret_cast<uint8_t*>(tile + (a.dbias ? 2 * LGT_STRIDE : 0));
     uint32_t at = blockIdx.x;
-    const int v0 = (int)(at % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0), end = n * a.inner;
+    const int v0 = (int)(at % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0), end = n * a.inner, words = (n + 31) >> 5;
     at /= a.chunks;
     const int r = (int)(at % a.bias_rows), part = (int)(at / a.bias_rows), many = a.rows / a.bias_rows;
     const int first = (int)((long long)many * part / a.splits), last = (int)((long long)many * (part + 1) / a.splits);
@@ -385,64 +397,105 @@ __global__ __launch_bounds__(LGT_THREADS) void k_scores_bwd(LogitsArgs a) {
     // lanes that add one entry's elements: a power of two, so that they lie in one wavefront
     int group = 1;
     while (group < 64 && group * 2 * n <= LGT_THREADS) group *= 2;
-    const int mine = threadIdx.x / group, member = threadIdx.x % group;
-    float sum[LGT_PER_LANE] = {};
-    for (int q = first; q < last; ++q) {
-        const int o = r + q * a.bias_rows, mask_row = a.mask_type ? o % a.mask_rows : 0;
-        const float rho = lgt_param(a.rep, a.rep_rows, a.rep_value, o), inv_rho = 1.f / rho;
-        const float inv_tau = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
-        if (a.history) lgt_count<false>(a, o, lgt_first_ids(a, o % a.history_rows), v0, n, cnt);
-        for (int v = threadIdx.x; v < n; v += LGT_THREADS)
-            cnt[v] = (a.history && cnt[v] ? LGT_SEEN : 0) | (lgt_on(a, mask_row, v0 + v) ? 0 : LGT_OFF);
-        __syncthreads();
-        const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + (long long)v0 * a.inner;
-        const T* dy = static_cast<const T*>(a.dy) + (long long)o * a.y_stride + (long long)v0 * a.inner;
-        T* dx = a.y ? static_cast<T*>(a.y) + (long long)o * a.y_stride + (long long)v0 * a.inner : nullptr;
-        for (int e = threadIdx.x * LGT_PER_LANE; e < end; e += LGT_STRIDE) {
-            const int left = end - e;
-            const LgtVec<T, LGT_PER_LANE> raw = lgt_load(dy, e, left);
-            float g[LGT_PER_LANE];
-            uint32_t c[LGT_PER_LANE], any = 0;
-            int v = n == 1 ? 0 : lgt_entry(e, inv_inner), i = e - v * a.inner;
-#pragma unroll
-            for (int k = 0; k < LGT_PER_LANE; ++k) {
-                c[k] = cnt[min(v, n - 1)];
-                any |= c[k];
-                g[k] = c[k] & LGT_OFF ? 0.f : (float)raw[k] * inv_tau;
-                if (++i == a.inner) { i = 0; ++v; }
+    const int mine = threadIdx.x / group, member = threadIdx.x % group, entries = LGT_THREADS / group;
+    const int w = a.history_wide ? 2 : 4, groups = a.history ? (int)((a.history_len + w - 1) / w) : 1;
+    const int e0 = threadIdx.x * LGT_PER_LANE;
+    const int lane_v = n == 1 ? 0 : lgt_entry(min(e0, end), inv_inner), lane_i = e0 - lane_v * a.inner;
+    float sum[LGT_SCORE_ENTRIES / LGT_THREADS] = {};
+    for (int q = first; q < last; q += LGT_SCORE_ROWS) {
+        const int rows = min(LGT_SCORE_ROWS, last - q);
+        const auto row_of = [&](int j) { return r + (q + j) * a.bias_rows; };
+        const auto dy_of = [&](int j) { return static_cast<const T*>(a.dy) + (long long)row_of(j) * a.y_stride + (long long)v0 * a.inner; };
+        LgtVec<T, LGT_PER_LANE> next = lgt_load(dy_of(0), e0, end - e0);
+        if (q != first) __syncthreads();
+        if ((int)threadIdx.x < rows) {
+            const int o = row_of(threadIdx.x);
+            slope[threadIdx.x][0] = 1.f / lgt_param(a.temp, a.temp_rows, a.temp_value, o);
+            slope[threadIdx.x][1] = lgt_param(a.rep, a.rep_rows, a.rep_value, o);
+            if (a.history) {
+                const long long len = a.lens ? lgt_int(a.lens, a.lens_wide, o % a.history_rows) : a.history_len;
+                length[threadIdx.x] = (int)(len < 0 ? 0 : len < a.history_len ? len : a.history_len);
             }
-            if (a.dbias) lgt_store(tile, e, left, g);
-            if (dx) {
-                if (any & LGT_SEEN) {
-                    const LgtVec<T, LGT_PER_LANE> xs = lgt_load(x, e, left);
-#pragma unroll
-                    for (int k = 0; k < LGT_PER_LANE; ++k)
-                        if (c[k] == LGT_SEEN) g[k] *= (float)xs[k] > 0.f ? inv_rho : rho;
-                }
-                lgt_store(dx, e, left, g);
+        }
+        if (a.history) {
+            for (int k = threadIdx.x; k < rows * words; k += LGT_THREADS) seen[k] = 0;
+            __syncthreads();
+            const int step_row = LGT_THREADS / groups, step_group = LGT_THREADS % groups;
+            int j = threadIdx.x / groups, g = threadIdx.x % groups;
+            while (j < rows) {
+                const int len = length[j], l = g * w;
+                const long long base = (long long)(row_of(j) % a.history_rows) * a.history_len + l;
+                for (int k = 0; k < w && l + k < len; ++k) lgt_see(lgt_int(a.history, a.history_wide, base + k), v0, n, seen + j * words);
+                j += step_row;
+                g += step_group;
+                if (g >= groups) { g -= groups; ++j; }
+            }
+            __syncthreads();
+        }
+        {
+            const int step_row = LGT_THREADS / n, step_v = LGT_THREADS % n;
+            int j = threadIdx.x / n, v = threadIdx.x % n;
+            while (j < rows) {
+                const bool was = a.history && (seen[j * words + (v >> 5)] >> (v & 31) & 1);
+                flag[j * n + v] = (was ? 1 : 0) | (lgt_on(a, a.mask_type ? row_of(j) % a.mask_rows : 0, v0 + v) ? 0 : 2);
+                j += step_row;
+                v += step_v;
+                if (v >= n) { v -= n; ++j; }
             }
         }
         __syncthreads();
-        if (a.dbias) {
-            // entries mine, mine + 512 / group, ...: at most 8 passes, as a tile has at most 4096 elements in at most 2048 entries
+        for (int j = 0; j < rows; ++j) {
+            const float inv_tau = slope[j][0], rho = slope[j][1], inv_rho = 1.f / rho;
+            const T* x = static_cast<const T*>(a.x) + (long long)row_of(j) * a.x_stride + (long long)v0 * a.inner;
+            T* dx = a.y ? static_cast<T*>(a.y) + (long long)row_of(j) * a.y_stride + (long long)v0 * a.inner : nullptr;
+            float* out = tile + (j & 1) * LGT_STRIDE;
+            LgtVec<T, LGT_PER_LANE> raw = next;
+            if (j + 1 < rows) next = lgt_load(dy_of(j + 1), e0, end - e0);
+            for (int e = e0; e < end; e += LGT_STRIDE) {
+                const int left = end - e;
+                if (e != e0) raw = lgt_load(dy_of(j), e, left);
+                float g[LGT_PER_LANE];
+                uint32_t was = 0;                                             // bit k: seen, and on
+                int v = e == e0 ? lane_v : 0, i = e == e0 ? lane_i : 0;       // more than one stride: one entry
 #pragma unroll
-            for (int p = 0; p < LGT_PER_LANE; ++p) {
-                const int v = mine + p * (LGT_THREADS / group);
-                float s = 0.f;
-                if (v < n)
-                    for (int i = member; i < a.inner; i += group) s += tile[v * a.inner + i];
-                for (int off = group >> 1; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
-                sum[p] += s;
-                if ((p + 1) * (LGT_THREADS / group) >= n) break;
+                for (int k = 0; k < LGT_PER_LANE; ++k) {
+                    const uint32_t c = flag[j * n + min(v, n - 1)];
+                    was |= (c == 1 ? 1u : 0u) << k;
+                    g[k] = c & 2 ? 0.f : (float)raw[k] * inv_tau;
+                    if (++i == a.inner) { i = 0; ++v; }
+                }
+                if (a.dbias) lgt_store(out, e, left, g);
+                if (dx) {
+                    if (was) {
+                        const LgtVec<T, LGT_PER_LANE> xs = lgt_load(x, e, left);
+#pragma unroll
+                        for (int k = 0; k < LGT_PER_LANE; ++k)
+                            if (was >> k & 1) g[k] *= (float)xs[k] > 0.f ? inv_rho : rho;
+                    }
+                    lgt_store(dx, e, left, g);
+                }
             }
-            __syncthreads();
+            if (a.dbias) {
+                __syncthreads();
+                // entries mine, mine + entries, ...: at most 4 passes, as a tile has at most 2048 entries
+                for (int p = 0; p < LGT_SCORE_ENTRIES / LGT_THREADS; ++p) {
+                    const int v = mine + p * entries;
+                    float s = 0.f;
+                    if (v < n)
+                        for (int i = member; i < a.inner; i += group) s += out[v * a.inner + i];
+                    for (int off = group >> 1; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
+#pragma unroll
+                    for (int z = 0; z < LGT_SCORE_ENTRIES / LGT_THREADS; ++z) sum[z] += z == p ? s : 0.f;
+                    if ((p + 1) * entries >= n) break;
+                }
+            }
         }
     }
     if (a.dbias && member == 0) {
         float* out = a.dbias + ((long long)part * a.bias_rows + r) * a.vocab + v0;
 #pragma unroll
-        for (int p = 0; p < LGT_PER_LANE; ++p) {
-            const int v = mine + p * (LGT_THREADS / group);
+        for (int p = 0; p < LGT_SCORE_ENTRIES / LGT_THREADS; ++p) {
+            const int v = mine + p * entries;
             if (v < n) out[v] = sum[p];
         }
     }

@@ -66,15 +66,15 @@ int fill_args(const gcn_logits_desc* d, LogitsArgs* a) {
     return 0;
 }
 
-size_t lds_of(const LogitsArgs& a, bool with_add, bool with_tile) {
+size_t lds_of_fwd(const LogitsArgs& a) {
     if (a.inner == 1) return a.history ? (size_t)a.chunk * sizeof(uint32_t) : 0;
-    return ((size_t)((a.chunk + 3) & ~3) + (with_add ? a.chunk : 0) + (with_tile ? LGT_STRIDE : 0)) * sizeof(uint32_t);
+    return (size_t)(((a.chunk + 3) & ~3) + a.chunk) * sizeof(uint32_t);
 }
 
 template <typename T>
 int launch_fwd(const LogitsArgs& a, hipStream_t st) {
     const uint32_t blocks = (uint32_t)a.rows * a.chunks;
-    const size_t lds = lds_of(a, true, false);
+    const size_t lds = lds_of_fwd(a);
     GCN_PROF_PRE(a.inner == 1 ? "k_logits" : "k_scores");
     const bool wide = a.chunk == 2 * LGT_STRIDE, far = a.history && a.history_len >= 8192;
     if (a.inner > 1) k_scores<T><<<blocks, LGT_THREADS, lds, st>>>(a);
@@ -93,14 +93,12 @@ void set_bwd_chunk(LogitsArgs* a) {
     a->chunks = (a->vocab + a->chunk - 1) / a->chunk;
 }
 
-// Parts of the rows that share a bias row: about 1024 workgroups, but sums of the parts (written and read in fp32) of at most
-// an eighth of the gradient's bytes where that is more than a launch's worth.
+// Parts of the rows that share a bias row: about 1024 workgroups, but with several rows each where there are enough (a turn's
+// histories are counted together; 800 rows of 200 x 100 scores in fp32: 33 us with 4 rows, 41 with 2, 59 with 1), and sums of the
+// parts (written and read in fp32) of at most an eighth of the gradient's bytes where that is more than a launch's worth.
 int splits_of(const LogitsArgs& a, bool want_bias, int type) {
     const long long many = a.rows / a.bias_rows, per_part = (long long)a.chunks * a.bias_rows;
-    if (!want_bias && a.inner > 1) return (int)many;
-    long long target = 1024;
-    if (const char* e = tune_env("GCN_TUNE_LOGITS_WG")) target = atoi(e);
-    long long splits = std::min(many, (target + per_part - 1) / per_part);
+    const long long splits = std::max(1ll, std::min(many, 1024 / per_part));
     if (!want_bias) return (int)splits;
     const long long data = (long long)a.rows * a.vocab * a.inner * (type == GCN_F32 ? 8 : 4), part = 8ll * a.bias_rows * a.vocab;
     return (int)std::max(1ll, std::min(splits, std::max(data, 32ll << 20) / 8 / part));
@@ -114,7 +112,7 @@ int launch_bwd(LogitsArgs a, float* dbias, int splits, float* parts, hipStream_t
     a.dbias = by_tile ? (splits > 1 ? parts : dbias) : nullptr;
     if ((long long)a.chunks * a.bias_rows * splits > 0x7fffffffll) return fail(-2, "gcn_logits_process_bwd: too many rows");
     const uint32_t blocks = (uint32_t)((long long)a.chunks * a.bias_rows * splits);
-    const size_t lds = lds_of(a, false, by_tile);
+    const size_t lds = (by_tile ? 2 * LGT_STRIDE * sizeof(float) : 0) + (size_t)LGT_SCORE_ROWS * a.chunk;
     if (a.y || by_tile) {
         GCN_PROF_PRE(a.inner == 1 ? "k_logits_bwd" : "k_scores_bwd");
         if (a.inner > 1) k_scores_bwd<T><<<blocks, LGT_THREADS, lds, st>>>(a);
