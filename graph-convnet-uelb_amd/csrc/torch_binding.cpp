@@ -83,37 +83,39 @@ struct List {
         if (!held) throw py::error_already_set();
         const Py_ssize_t n = PySequence_Fast_GET_SIZE(held.ptr());
         PyObject** items = PySequence_Fast_ITEMS(held.ptr());
-        t.reserve(n);
+        t.resize(n);
         for (Py_ssize_t k = 0; k < n; ++k) {
-            const at::Tensor* x = as_tensor(items[k]);
-            if (!x) type_error(name, " is a list of tensors");
-            t.push_back(x);
+            t[k] = as_tensor(items[k]);
+            if (!t[k]) type_error(name, " is a list of tensors");
         }
     }
     // as many tensors as `sizes`, of these sizes (or as many blocks of them) and this type, contiguous
     void check(const std::vector<int64_t>& sizes, at::ScalarType type, int64_t block = 1) {
         if (t.size() != sizes.size()) value_error(t.size(), " tensors in ", name, " for ", sizes.size(), " parameters");
         for (size_t k = 0; k < t.size(); ++k) {
-            if (t[k]->numel() != (sizes[k] + block - 1) / block) value_error("the tensors in ", name, " do not have the parameters' sizes");
-            if (t[k]->scalar_type() != type) type_error(name, " holds ", t[k]->scalar_type(), " (expected ", type, ")");
-            if (!t[k]->is_contiguous()) value_error(name, " needs contiguous tensors");
+            const at::TensorImpl* x = t[k]->unsafeGetTensorImpl();
+            if (x->numel() != (block == 1 ? sizes[k] : (sizes[k] + block - 1) / block)) value_error("the tensors in ", name, " do not have the parameters' sizes");
+            if (x->dtype() != at::scalarTypeToTypeMeta(type)) type_error(name, " holds ", t[k]->scalar_type(), " (expected ", type, ")");
+            if (!x->is_contiguous()) value_error(name, " needs contiguous tensors");
         }
     }
-    void on(c10::Device d) {
-        for (const at::Tensor* x : t) {
-            need_gpu(*x, "tensor");
-            if (x->device() != d) value_error("the tensors of one call are on one GPU");
-        }
-    }
-    // addresses for the library; of tensors that it writes, autograd hears too
-    void* const* place(bool written) {
+    // all on that GPU; their addresses for the library
+    void place(c10::Device d, bool written) {
         ptr.resize(t.size());
         for (size_t k = 0; k < t.size(); ++k) {
+            if (t[k]->device() != d) {
+                need_gpu(*t[k], "tensor");
+                value_error("the tensors of one call are on one GPU");
+            }
             ptr[k] = written ? t[k]->mutable_data_ptr() : const_cast<void*>(t[k]->const_data_ptr());
-            if (written && !t[k]->is_inference()) t[k]->unsafeGetTensorImpl()->bump_version();
         }
-        return given ? ptr.data() : nullptr;
     }
+    // autograd hears of what was written
+    void written() const {
+        for (const at::Tensor* x : t)
+            if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+    }
+    void* const* table() const { return given ? ptr.data() : nullptr; }
 };
 
 const float* device_scalar(py::handle h, const char* name, c10::Device d) {
@@ -158,7 +160,8 @@ void adamw_step(py::handle params_, py::handle grads_, py::handle exp_avgs_, py:
     }
     if (params.t.empty()) return;
     const c10::Device d = params.t[0]->device();
-    for (List* l : {&params, &grads, &m, &v, &masters, &em, &ev}) l->on(d);
+    need_gpu(*params.t[0], "tensor");
+    for (List* l : {&params, &grads, &m, &v, &masters, &em, &ev}) l->place(d, l != &grads);
     const void* hyper = nullptr;
     if (!hyper_.is_none()) {
         const at::Tensor* t = as_tensor(hyper_);
@@ -178,11 +181,11 @@ void adamw_step(py::handle params_, py::handle grads_, py::handle exp_avgs_, py:
     desc.step = step;
     desc.seed = seed;
     static_assert(sizeof(long long) == sizeof(int64_t), "sizes are handed over as they are");
-    check(api.adamw_step(&desc, params.place(true), grads.place(false), reinterpret_cast<float* const*>(half ? masters.place(true) : nullptr),
-                         m.place(true), v.place(true), reinterpret_cast<unsigned char* const*>(em.place(true)),
-                         reinterpret_cast<unsigned char* const*>(ev.place(true)), reinterpret_cast<const long long*>(sizes.data()), scale, clip, hyper,
-                         stream_of(d)),
+    check(api.adamw_step(&desc, params.table(), grads.table(), reinterpret_cast<float* const*>(masters.table()), m.table(), v.table(),
+                         reinterpret_cast<unsigned char* const*>(em.table()), reinterpret_cast<unsigned char* const*>(ev.table()),
+                         reinterpret_cast<const long long*>(sizes.data()), scale, clip, hyper, stream_of(d)),
           "gcn_adamw_step");
+    for (const List* l : {&params, &m, &v, &masters, &em, &ev}) l->written();
 }
 
 py::tuple grad_norm(py::handle grads_, py::handle max_norm_, py::handle grad_scale) {
@@ -195,7 +198,8 @@ py::tuple grad_norm(py::handle grads_, py::handle max_norm_, py::handle grad_sca
     const std::vector<int64_t> sizes = sizes_of(grads);
     grads.check(sizes, type);
     const c10::Device d = grads.t[0]->device();
-    grads.on(d);
+    need_gpu(*grads.t[0], "tensor");
+    grads.place(d, false);
     const float* scale = device_scalar(grad_scale, "grad_scale", d);
     c10::DeviceGuard guard(d);
     const int n = static_cast<int>(sizes.size());
@@ -203,7 +207,7 @@ py::tuple grad_norm(py::handle grads_, py::handle max_norm_, py::handle grad_sca
     const size_t bytes = api.grad_norm_ws_bytes(n, numel);
     at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(d));
     at::Tensor out = at::empty({2}, at::TensorOptions().dtype(at::kFloat).device(d));
-    check(api.grad_norm(n, type_id(type), reinterpret_cast<const void* const*>(grads.place(false)), numel, scale, max_norm,
+    check(api.grad_norm(n, type_id(type), reinterpret_cast<const void* const*>(grads.table()), numel, scale, max_norm,
                         static_cast<float*>(out.mutable_data_ptr()), ws.mutable_data_ptr(), bytes, stream_of(d)),
           "gcn_grad_norm");
     return py::make_tuple(out.select(0, 0), clip ? py::cast(out.select(0, 1)) : py::none());
