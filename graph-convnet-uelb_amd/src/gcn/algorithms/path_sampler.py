@@ -171,6 +171,13 @@ class PathSampler:
         is_feasible = bool((max_lf <= 1.0).all().item())
         return batch_paths, logp_b, is_feasible, entropies
 
+    def draw(self):
+        """Paths only, on the device: (paths int32 [B, C, max(V, 10)], path_len int32 [B, C]); no gradient, no copy to the host."""
+        with torch.no_grad():
+            _, paths, plen, *_ = PathLogProbFn.apply(self.y_pred_edges.detach().float().contiguous(), self._cap, self._comm, float(self.temperature),
+                                                     float(self.top_p), float(self.entropy_epsilon), _rng_words(self.device), None)
+        return paths, plen
+
     def sample(self):
         """Returns (batch_paths[b][c], log_probs_tensor [B], is_feasible, batch_stepwise_entropies[b][c][step])."""
         return self._finish(*self._run())

@@ -22,11 +22,24 @@ import torch
 from ...common.data_management.dataset_reader import DatasetReader
 from ..hip import dist as D
 from ..hip.fused_adam import FusedAdam
+from ..hip.fused_adamw import FusedAdamW
 from ..hip.train_step import HipTrainStep
 from ..models.gcn_model import ResidualGatedGCNModel
 from ..models.model_utils import update_learning_rate
 from ..training.reinforcement_strategy import ReinforcementLearningStrategy
 from ..training.supervised_strategy import SupervisedLearningStrategy
+
+
+def make_optimizer(config, params):
+    """The optimizer of ``config['optimizer']``: 'adam' (the reference's torch.optim.Adam(lr), trainer.py:95, and the default), or
+    'adamw' / 'adamw8bit' (FusedAdamW with moments in 32 or 8 bits) with 'weight_decay' (0.01) and 'max_grad_norm' (none)."""
+    kind = config.get('optimizer', 'adam')
+    if kind == 'adam':
+        return FusedAdam(params, lr=config.learning_rate)
+    if kind not in ('adamw', 'adamw8bit'):
+        raise ValueError(f"Unknown optimizer: {kind!r} (expected 'adam', 'adamw' or 'adamw8bit')")
+    return FusedAdamW(params, lr=config.learning_rate, weight_decay=config.get('weight_decay', 0.01),
+                      state_bits=8 if kind == 'adamw8bit' else 32, max_grad_norm=config.get('max_grad_norm', None))
 
 
 class Trainer:
@@ -44,7 +57,7 @@ class Trainer:
                                  convert_supervised_to_rl=bool(config.get('convert_supervised_to_rl', False)))
         D.broadcast_parameters(self.net.parameters())
         # the reference builds torch.optim.Adam(lr) here (trainer.py:95); same arithmetic and state layout, one launch per step
-        self.optimizer = FusedAdam(self.net.parameters(), lr=config.learning_rate)
+        self.optimizer = make_optimizer(config, self.net.parameters())
         strategy_type = config.get('training_strategy', 'supervised')
         if strategy_type == 'supervised':
             self.strategy = SupervisedLearningStrategy(config)

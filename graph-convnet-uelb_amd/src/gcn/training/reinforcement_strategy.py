@@ -18,7 +18,9 @@ from ..hip import dist as D
 from ...common.graph.graph_utils import load_factor_from_tensors
 from ..algorithms.beamsearch_uelb import BeamSearchFactory
 from ..algorithms.path_sampler import PathSampler
+from ..algorithms.score_rules import LinkScoreRules
 from ..hip import lib as L
+from ..hip.fused_adamw import FusedAdamW, grad_norm
 from .base_strategy import BaseTrainingStrategy
 
 
@@ -96,6 +98,10 @@ class ReinforcementLearningStrategy(BaseTrainingStrategy):
         self.grad_norm_history_size = g('rl_grad_norm_history_size', 100)
         self.grad_clip_max_norm = g('rl_grad_clip_max_norm', 1.0)
         self.last_grad_explosion = False
+        # penalties for links that a first draw of all commodities uses, applied to the scores before the paths that count are
+        # drawn (LinkScoreRules); neutral by default: one draw on the scores as they are
+        self.link_penalties = dict(repetition_penalty=g('rl_link_repetition_penalty', 1.0), presence_penalty=g('rl_link_presence_penalty', 0.0),
+                                   frequency_penalty=g('rl_link_frequency_penalty', 0.0))
         # test hook: (paths int32 [B,C,PL], path_len int32 [B,C]) to evaluate instead of sampling
         self.replay_paths = None
 
@@ -129,6 +135,11 @@ class ReinforcementLearningStrategy(BaseTrainingStrategy):
         if sampling:
             if y_preds.dim() != 4:
                 raise ValueError("path sampling needs edge scores [B,V,V,C] (voc_edges_out == 1)")
+            if list(self.link_penalties.values()) != [1.0, 0.0, 0.0]:
+                first = PathSampler(y_pred_edges=y_preds, edges_capacity=cap, commodities=comm, num_samples=1,
+                                    temperature=self.get_current_temperature(), top_p=self.sampling_top_p,
+                                    entropy_epsilon=self.entropy_epsilon).draw()
+                y_preds = LinkScoreRules(cap, **self.link_penalties)(y_preds, *first)
             sampler = PathSampler(y_pred_edges=y_preds, edges_capacity=cap, commodities=comm, num_samples=1,
                                   temperature=self.get_current_temperature(), top_p=self.sampling_top_p,
                                   entropy_epsilon=self.entropy_epsilon)
@@ -249,8 +260,15 @@ class ReinforcementLearningStrategy(BaseTrainingStrategy):
             # Over the fixed parameter list (zeros for a missing .grad), so that every rank sends the same message
             D.allreduce_mean_grads(every)
         params = [p for p in every if p.grad is not None]
-        with torch.no_grad():
-            total = torch.linalg.vector_norm(torch.stack([p.grad.norm() for p in params])).item() if params else 0.0
+        fused, stepped = isinstance(optimizer, FusedAdamW) and bool(params), False
+        if fused and last_micro_step and self.grad_clip_max_norm > 0:
+            optimizer.step(max_grad_norm=self.grad_clip_max_norm)        # norm, clipping and update in the optimizer's launches
+            total, stepped = optimizer.grad_norm.item(), True
+        elif fused and len({p.dtype for p in params}) == 1:
+            total = grad_norm([p.grad.contiguous() for p in params])[0].item()
+        else:
+            with torch.no_grad():
+                total = torch.linalg.vector_norm(torch.stack([p.grad.norm() for p in params])).item() if params else 0.0
         # the history the explosion detector looks at holds averaged gradients only: under several ranks the norm of
         # a micro-step before the all-reduce is a local one and would differ from rank to rank
         if last_micro_step or not D.active() or D.world() == 1:
@@ -266,9 +284,10 @@ class ReinforcementLearningStrategy(BaseTrainingStrategy):
         if not np.isfinite(total):
             print(f"warning: non-finite gradient norm {total}", flush=True)
         if (batch_num + 1) % accumulation_steps == 0:
-            if self.grad_clip_max_norm > 0 and params:
-                torch.nn.utils.clip_grad_norm_(params, self.grad_clip_max_norm)
-            optimizer.step()
+            if not stepped:
+                if self.grad_clip_max_norm > 0 and params:
+                    torch.nn.utils.clip_grad_norm_(params, self.grad_clip_max_norm)
+                optimizer.step()
             optimizer.zero_grad()
             return True
         return False
