@@ -43,7 +43,10 @@ struct LogitsArgs {
     float rep_value, pres_value, freq_value, temp_value, masked_value;
     int splits;                    // backward: parts of the rows that share a bias row
     float* dbias;                  // backward: [splits][bias_rows][vocab] or null
+    uint32_t blocks;               // workgroups, over both dimensions of the grid (a dimension holds 2^32 threads)
 };
+
+__device__ __forceinline__ uint32_t lgt_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
 __device__ __forceinline__ float lgt_param(const float* p, int rows, float value, int o) { return p ? p[rows == 1 ? 0 : o % rows] : value; }
 __device__ __forceinline__ long long lgt_int(const void* p, int wide, long long i) {
@@ -173,7 +176,8 @@ __device__ __forceinline__ void lgt_store(T* p, long long e, int left, const flo
 template <typename T, int ITER, bool LONG>
 __global__ __launch_bounds__(LGT_THREADS) void k_logits(LogitsArgs a) {
     extern __shared__ __align__(16) uint32_t cnt[];
-    const int o = blockIdx.x / a.chunks, v0 = (blockIdx.x % a.chunks) * (ITER * LGT_STRIDE), n = min(ITER * LGT_STRIDE, a.vocab - v0);
+    if (lgt_block() >= a.blocks) return;
+    const int o = lgt_block() / a.chunks, v0 = (lgt_block() % a.chunks) * (ITER * LGT_STRIDE), n = min(ITER * LGT_STRIDE, a.vocab - v0);
     const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + v0;
     T* y = static_cast<T*>(a.y) + (long long)o * a.y_stride + v0;
     const int mask_row = a.mask_type ? o % a.mask_rows : 0;
@@ -241,7 +245,8 @@ __global__ __launch_bounds__(LGT_THREADS) void k_logits_bwd(LogitsArgs a) {
     __shared__ uint32_t bits[LGT_ROWS * WORDS];
     __shared__ float slope[LGT_ROWS][2];         // 1 / temperature and repetition penalty of the rows
     __shared__ int length[LGT_ROWS];
-    uint32_t at = blockIdx.x;
+    uint32_t at = lgt_block();
+    if (at >= a.blocks) return;
     const int v0 = (int)(at % a.chunks) * LGT_STRIDE, n = min(LGT_STRIDE, a.vocab - v0);
     at /= a.chunks;
     const int r = (int)(at % a.bias_rows), part = (int)(at / a.bias_rows), many = a.rows / a.bias_rows;
@@ -336,7 +341,8 @@ __device__ __forceinline__ int lgt_entry(int e, float inv_inner) { return (int)(
 template <typename T>
 __global__ __launch_bounds__(LGT_THREADS) void k_scores(LogitsArgs a) {
     extern __shared__ __align__(16) uint32_t cnt[];
-    const int o = blockIdx.x / a.chunks, v0 = (blockIdx.x % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0);
+    if (lgt_block() >= a.blocks) return;
+    const int o = lgt_block() / a.chunks, v0 = (lgt_block() % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0);
     float* add = reinterpret_cast<float*>(cnt + ((a.chunk + 3) & ~3));
     const T* x = static_cast<const T*>(a.x) + (long long)o * a.x_stride + (long long)v0 * a.inner;
     T* y = static_cast<T*>(a.y) + (long long)o * a.y_stride + (long long)v0 * a.inner;
@@ -388,7 +394,8 @@ __global__ __launch_bounds__(LGT_THREADS) void k_scores_bwd(LogitsArgs a) {
     __shared__ int length[LGT_SCORE_ROWS];
     extern __shared__ __align__(16) float tile[];             // with dbias: two of LGT_STRIDE elements; then a flag per (row, entry)
     uint8_t* flag = reinterpret_cast<uint8_t*>(tile + (a.dbias ? 2 * LGT_STRIDE : 0));
-    uint32_t at = blockIdx.x;
+    uint32_t at = lgt_block();
+    if (at >= a.blocks) return;
     const int v0 = (int)(at % a.chunks) * a.chunk, n = min(a.chunk, a.vocab - v0), end = n * a.inner, words = (n + 31) >> 5;
     at /= a.chunks;
     const int r = (int)(at % a.bias_rows), part = (int)(at / a.bias_rows), many = a.rows / a.bias_rows;

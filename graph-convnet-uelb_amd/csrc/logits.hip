@@ -71,9 +71,16 @@ size_t lds_of_fwd(const LogitsArgs& a) {
     return (size_t)(((a.chunk + 3) & ~3) + a.chunk) * sizeof(uint32_t);
 }
 
+// As many workgroups in two dimensions: one of them holds less than 2^32 threads.
+dim3 grid_of(uint32_t blocks) {
+    const uint32_t x = std::min(blocks, 1u << 22);
+    return dim3(x, (blocks + x - 1) / x);
+}
+
 template <typename T>
-int launch_fwd(const LogitsArgs& a, hipStream_t st) {
-    const uint32_t blocks = (uint32_t)a.rows * a.chunks;
+int launch_fwd(LogitsArgs a, hipStream_t st) {
+    a.blocks = (uint32_t)a.rows * a.chunks;
+    const dim3 blocks = grid_of(a.blocks);
     const size_t lds = lds_of_fwd(a);
     GCN_PROF_PRE(a.inner == 1 ? "k_logits" : "k_scores");
     const bool wide = a.chunk == 2 * LGT_STRIDE, far = a.history && a.history_len >= 8192;
@@ -111,7 +118,8 @@ int launch_bwd(LogitsArgs a, float* dbias, int splits, float* parts, hipStream_t
     a.splits = splits;
     a.dbias = by_tile ? (splits > 1 ? parts : dbias) : nullptr;
     if ((long long)a.chunks * a.bias_rows * splits > 0x7fffffffll) return fail(-2, "gcn_logits_process_bwd: too many rows");
-    const uint32_t blocks = (uint32_t)((long long)a.chunks * a.bias_rows * splits);
+    a.blocks = (uint32_t)((long long)a.chunks * a.bias_rows * splits);
+    const dim3 blocks = grid_of(a.blocks);
     const size_t lds = (by_tile ? 2 * LGT_STRIDE * sizeof(float) : 0) + (size_t)LGT_SCORE_ROWS * a.chunk;
     if (a.y || by_tile) {
         GCN_PROF_PRE(a.inner == 1 ? "k_logits_bwd" : "k_scores_bwd");

@@ -11,6 +11,8 @@ namespace {
 
 constexpr uint64_t kNormSpan = OPT_NORM_UNITS * OPT_STRIDE;       // elements of a workgroup of k_grad_norm
 
+constexpr uint64_t kMostBlocks = 0xffffffffull / OPT_THREADS;       // workgroups of a launch: less than 2^32 threads
+
 int log2_of(uint64_t power) { return __builtin_ctzll(power); }
 
 // Elements of a workgroup of k_adamw: one stride of 2048; two with 8-bit states, where the search for the tensor weighs more,
@@ -110,7 +112,7 @@ int gcn_adamw_step(const gcn_adamw_desc* d, void* const* params, const void* con
         // tensors keep their numbers: an empty one takes a place without workgroups
         for (; k < d->n && t.n < t.cap; ++k, ++t.n) {
             const uint64_t more = units_of((uint64_t)numel[k], t.span);
-            if (blocks + more > 0x7fffffffull) {
+            if (blocks + more > kMostBlocks) {
                 if (t.n == 0) return fail(-2, "gcn_adamw_step: tensor %d is too large for one launch", k);
                 break;
             }
@@ -170,7 +172,7 @@ int gcn_grad_norm(int n, int type, const void* const* grads, const long long* nu
         uint64_t blocks = 0;
         for (; k < n && t.n < t.cap; ++k, ++t.n) {
             const uint64_t more = units_of((uint64_t)numel[k], kNormSpan);
-            if (blocks + more > 0x7fffffffull) {
+            if (blocks + more > kMostBlocks) {
                 if (t.n == 0) return fail(-2, "gcn_grad_norm: tensor %d is too large for one launch", k);
                 break;
             }

@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <sstream>
@@ -162,6 +163,12 @@ void adamw_step(py::handle params_, py::handle grads_, py::handle exp_avgs_, py:
     const c10::Device d = params.t[0]->device();
     need_gpu(*params.t[0], "tensor");
     for (List* l : {&params, &grads, &m, &v, &masters, &em, &ev}) l->place(d, l != &grads);
+    // a tensor twice would be updated by two workgroups at once
+    std::vector<void*> once;
+    for (size_t k = 0; k < sizes.size(); ++k)
+        if (sizes[k] > 0) once.push_back(params.ptr[k]);
+    std::sort(once.begin(), once.end());
+    if (std::adjacent_find(once.begin(), once.end()) != once.end()) value_error("a parameter is in the list twice");
     const void* hyper = nullptr;
     if (!hyper_.is_none()) {
         const at::Tensor* t = as_tensor(hyper_);
@@ -399,7 +406,7 @@ py::object process_logits(py::handle logits_, int64_t dim, py::handle history_, 
     const bool grad = at::GradMode::is_enabled() && (logits.requires_grad() || (bias && bias->requires_grad()));
     const at::Tensor* out = tensor_or_none(out_, "out");
     if (out) {
-        if (grad || out->requires_grad()) value_error("out does not go with gradients");
+        if (grad || (at::GradMode::is_enabled() && out->requires_grad())) value_error("out does not go with gradients");
         if (out->sizes() != logits.sizes() || out->scalar_type() != logits.scalar_type() || out->device() != logits.device())
             value_error("out is a tensor like the logits");
         const int64_t stride = row_stride(*out, r.dim);

@@ -560,3 +560,24 @@ def test_copied_and_pickled_optimizers_keep_their_options(dev, A):
     for x, y in zip(a, b):
         assert x is not y and torch.equal(x, y)
     assert len({id(st["step"]) for st in opt.state_dict()["state"].values()}) == 4
+
+
+def test_a_parameter_twice_is_refused(dev, A):
+    s, _ = make(A, dev, [100, 50], torch.float32, 32)
+    twice = {k: [ts[0], ts[0]] if ts else [] for k, ts in s.items()}
+    before = s["p"][0].clone()
+    with pytest.raises(ValueError, match="twice"):
+        call(A, twice)
+    assert torch.equal(s["p"][0], before)
+    empty, _ = make(A, dev, [0, 0], torch.float32, 32)
+    call(A, {k: [ts[0], ts[0]] if ts else [] for k, ts in empty.items()})
+
+
+def test_autograd_hears_of_the_update(dev, A):
+    p = torch.nn.Parameter(torch.ones(10, device=dev))
+    y = (p * p).sum()
+    opt = A.FusedAdamW([p])
+    p.grad = torch.ones(10, device=dev)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

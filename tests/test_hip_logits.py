@@ -324,3 +324,43 @@ def test_offsets_beyond_32_bits(dev):
     last = x[-3:].detach().requires_grad_()
     (ref,) = torch.autograd.grad(process_logits(last, history=hist[-3:], **kind), [last], y[-3:].detach())
     assert torch.equal(dx[-3:], ref)
+
+
+def test_empty_logits_and_their_gradients(dev):
+    from src.gcn.hip.logits import process_logits
+    for shape in ((0, 8), (3, 0, 8), (4, 8, 0)):
+        x = torch.zeros(shape, device=dev, requires_grad=True)
+        b = torch.zeros(8, device=dev, requires_grad=True)
+        y = process_logits(x, dim=len(shape) - (2 if shape[-1] == 0 else 1), bias=b)
+        assert y.shape == x.shape
+        dx, db = torch.autograd.grad(y.sum(), [x, b])
+        assert dx.shape == x.shape and not bool(db.any())
+
+
+def test_in_place_without_gradients_on_a_tensor_that_needs_them(dev):
+    from src.gcn.hip.logits import process_logits
+    x = torch.randn(3, 8, device=dev, requires_grad=True)
+    y = x * 2
+    z = (y * y).sum()
+    with torch.no_grad():
+        want = process_logits(y, temperature=2.0)
+        assert process_logits(y, temperature=2.0, out=y) is y and torch.equal(y, want)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    with torch.inference_mode():
+        w = torch.randn(3, 8, device=dev)
+        ref = process_logits(w, temperature=2.0)
+        assert torch.equal(process_logits(w, temperature=2.0, out=w), ref)
+
+
+def test_more_workgroups_than_one_grid_dimension(dev):
+    """2^23 rows of a few entries: more than 2^32 threads of 512 in one dimension."""
+    from src.gcn.hip.logits import process_logits
+    rows, vocab = (1 << 23) + 5, 3
+    x = torch.randn(rows, vocab, device=dev, generator=torch.Generator(dev).manual_seed(0))
+    bias = torch.randn(rows, vocab, device=dev)
+    z, b = x.requires_grad_(), bias.requires_grad_()
+    y = process_logits(z, bias=b, temperature=0.5)
+    assert torch.equal(y, (x + bias) * 2)
+    dx, db = torch.autograd.grad(y, [z, b], torch.ones_like(y))
+    assert bool((dx == 2).all()) and bool((db == 2).all())
