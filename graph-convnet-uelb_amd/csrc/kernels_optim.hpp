@@ -18,7 +18,9 @@
 // and their neighbours are not touched.
 //
 // Bound by memory: 28 bytes per element with fp32 states, 16 with 8-bit states (fp32: p and g in, p out; with 16-bit
-// parameters master and g in, master and p out).
+// parameters master and g in, master and p out).  120 M bf16 parameters with fp32 states: 618 us, 5.4 TB/s, which is what the best
+// copy reaches; 159 M with 8-bit states: 501 us, 5.1 TB/s, the vector units busy 67 % of the time (76 instructions an
+// element); 129 tensors of 174 k elements in all: 5.7 us, one launch, bound by its chain of dependent loads.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -248,8 +250,8 @@ __device__ __forceinline__ void adamw_elements(const AdamwTensor<P>& w, uint64_t
         v = h.b2 * v + h.omb2 * (ge * ge);
         const float root = __builtin_sqrtf(v);
         const float below = root * h.inv_sqrt_bc2 + h.eps;
-        // 8 bits: the vector units are as busy as memory; the reciprocal (1 ulp, its argument is never near the ends of the
-        // range) saves 10 of 80 instructions an element
+        // 8 bits: the vector units are nearly as busy as memory; the reciprocal (1 ulp; `below` is at least eps, and below
+        // 1e28, whose reciprocal is normal; an eps under 2^-126 is as none) saves 10 instructions an element
         const float change = EIGHT ? m[e] * __builtin_amdgcn_rcpf(below) : m[e] / below;
         pi[e] = pi[e] * h.decay - h.step_size * change;
         r[e] = EIGHT ? root : v;
@@ -345,7 +347,8 @@ __global__ void k_adamw_advance(long long* __restrict__ step, const float* __res
 
 // Sum of squares of one unit of elements per workgroup, in double precision: no overflow or underflow of squares of finite
 // gradients, and no rounding that shows.  Every partial sum has a place of its own and the second kernel adds them in a fixed
-// order, so that equal gradients give equal bits.
+// order, so that equal gradients give equal bits.  Bound by memory: 300 tensors of 41 M fp32 elements in
+// all take 33 us with the final kernel, 5.0 TB/s, over gradients in turn; between steps of 41 M parameters 53 + 5 us.
 #define OPT_NORM_UNITS 4             // strides of a workgroup, all of them on the way at once
 template <typename P>
 __global__ __launch_bounds__(OPT_THREADS) void k_grad_norm(OptTable t, double* __restrict__ part) {
