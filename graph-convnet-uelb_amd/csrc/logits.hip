@@ -26,7 +26,8 @@ int fill_args(const gcn_logits_desc* d, LogitsArgs* a) {
     if (!d) return fail(-1, "gcn_logits: null descriptor");
     if (d->type < GCN_F32 || d->type > GCN_F16) return fail(-1, "gcn_logits: unknown type %d", d->type);
     if (d->rows < 0 || d->vocab < 1 || d->inner < 1) return fail(-1, "gcn_logits: %lld x %lld x %lld logits", d->rows, d->vocab, d->inner);
-    if (d->rows >= (1ll << 31) || d->vocab >= (1ll << 31) || d->inner >= (1ll << 31) || d->vocab * d->inner >= (1ll << 31) - 4096)
+    // 4096 below: the kernels step past the last row or element before they compare
+    if (d->rows >= (1ll << 31) - 4096 || d->vocab >= (1ll << 31) || d->inner >= (1ll << 31) || d->vocab * d->inner >= (1ll << 31) - 4096)
         return fail(-2, "gcn_logits: %lld x %lld x %lld logits are too many for 32-bit places in a row", d->rows, d->vocab, d->inner);
     if (d->in_stride < 0 || d->out_stride < d->vocab * d->inner) return fail(-1, "gcn_logits: row strides %lld, %lld", d->in_stride, d->out_stride);
     if (d->history && (d->history_len < 0 || d->history_len >= (1ll << 31) - LGT_THREADS)) return fail(-1, "gcn_logits: history of %lld", d->history_len);

@@ -130,3 +130,13 @@ def test_workspace_of_the_bias_gradient():
     assert ws(rows=2, vocab=4, inner=100000, out_stride=400000, bias=16, bias_rows=1) == 0
     d = L.LogitsDesc(**{**ok, "rows": 2000, "bias": 16, "bias_rows": 1})
     assert lib.gcn_logits_process_bwd(ctypes.byref(d), 16, 16, 16, 16, None, 0, None) == -2 and b"workspace" in lib.gcn_last_error()
+
+
+def test_rows_near_the_end_of_32_bits_are_refused():
+    """The backward kernels count rows in turns of 32: a count that starts below 2^31 must not pass it."""
+    lib = L.load()
+    one = dict(vocab=1, inner=1, in_stride=1, out_stride=1, type=2, repetition=1.0, temperature=1.0)
+    for rows, rc in (((1 << 31) - 1, -2), ((1 << 31) - 32, -2), ((1 << 31) - 4096, -2), ((1 << 31) - 4097, -1)):     # -1: the null pointers
+        d = L.LogitsDesc(rows=rows, **one)
+        assert lib.gcn_logits_process(ctypes.byref(d), None, None, None) == rc, rows
+        assert lib.gcn_logits_process_bwd(ctypes.byref(d), None, None, None, None, None, 0, None) == rc, rows
