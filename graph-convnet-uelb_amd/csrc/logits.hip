@@ -1,5 +1,6 @@
 // C ABI of the logits operators: argument checks and launches.  The entry points are documented in include/gcn_uelb_hip.h.
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 
 #include "../../include/gcn_uelb_hip.h"
@@ -12,6 +13,9 @@ int check_rows(const char* what, const void* p, long long n, long long rows) {
     if (p && (n < 1 || n > rows || rows % n)) return fail(-1, "gcn_logits: %lld rows of %s for %lld rows of logits", n, what, rows);
     return 0;
 }
+
+// A number whose reciprocal the kernels multiply by: with an infinite one, a logit of 0 would become NaN.
+bool divides(float x) { return x > 0.f && std::isfinite(x) && std::isfinite(1.f / x); }
 
 // Vocabulary of a workgroup of k_logits in strides of 4096 entries: two where that leaves 1024 workgroups, so that the history
 // is walked half as often (2048 rows of 32000: 65 us with two, 97 with one, 75 with four; 512 of 131072: 56, 82, 62; 1 of 32000:
@@ -33,8 +37,10 @@ int fill_args(const gcn_logits_desc* d, LogitsArgs* a) {
     if (d->history && (d->history_len < 0 || d->history_len >= (1ll << 31) - LGT_THREADS)) return fail(-1, "gcn_logits: history of %lld", d->history_len);
     if (!d->history && (d->history_lens || d->prompt_lens)) return fail(-1, "gcn_logits: lengths without a history");
     if (d->mask_type < 0 || d->mask_type > 2 || (d->mask_type != 0) != (d->mask != nullptr)) return fail(-1, "gcn_logits: mask of type %d", d->mask_type);
-    if (!d->repetition_t && !(d->repetition > 0.f)) return fail(-1, "gcn_logits: repetition penalty %g", (double)d->repetition);
-    if (!d->temperature_t && !(d->temperature > 0.f)) return fail(-1, "gcn_logits: temperature %g", (double)d->temperature);
+    if (!d->repetition_t && !divides(d->repetition)) return fail(-1, "gcn_logits: repetition penalty %g", (double)d->repetition);
+    if (!d->temperature_t && !divides(d->temperature)) return fail(-1, "gcn_logits: temperature %g", (double)d->temperature);
+    if ((!d->presence_t && !std::isfinite(d->presence)) || (!d->frequency_t && !std::isfinite(d->frequency)))
+        return fail(-1, "gcn_logits: presence penalty %g, frequency penalty %g", (double)d->presence, (double)d->frequency);
     const long long rows = std::max(d->rows, 1ll);
     if (d->rows > 0) {
         if (int rc = check_rows("history", d->history, d->history_rows, rows)) return rc;

@@ -283,7 +283,7 @@ void penalty(Rules& r, py::handle h, const char* name, const at::Tensor& logits,
     const double x = PyFloat_AsDouble(h.ptr());
     if (x == -1.0 && PyErr_Occurred()) throw py::error_already_set();
     *value = static_cast<float>(x);
-    if (!std::isfinite(x) || (positive && !(*value > 0.f))) value_error(name, " ", x);
+    if (!std::isfinite(*value) || (positive && !(*value > 0.f && std::isfinite(1.f / *value)))) value_error(name, " ", x);
 }
 
 at::Tensor run_forward(Rules& r, const at::Tensor& x, const at::Tensor& out) {

@@ -355,7 +355,8 @@ int gcn_grad_norm(int n, int type, const void* const* grads, const long long* nu
  *     x1 = seen ? (x > 0 ? x / repetition : x * repetition) : x
  *     y  = (x1 - n * frequency - (n > 0) * presence + bias[v]) / temperature,   masked_value where the mask has v off
  * Row o uses row o mod *_rows of each argument; *_rows divides rows.  repetition .. temperature: *_t (device, [*_rows])
- * or, where that is NULL, the number; repetition and temperature are positive.
+ * or, where that is NULL, the number; all are finite, repetition and temperature positive and with finite reciprocals
+ * (numbers are checked).
  * mask_type 1: uint8 [mask_rows][vocab], 0 = off; 2: 32-bit words [mask_rows][ceil(vocab / 32)], lowest bit first, 0 = off.
  * bias: float [bias_rows][vocab] or NULL.  A row whose mask leaves nothing becomes masked_value throughout.
  * gcn_logits_process_bwd: dout and din have out_stride; din (NULL: not wanted) and dbias [bias_rows][vocab] (NULL likewise) are

@@ -1,5 +1,6 @@
 """Rules on logits: refusals and host-side checks; no GPU needed."""
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -140,3 +141,22 @@ def test_rows_near_the_end_of_32_bits_are_refused():
         d = L.LogitsDesc(rows=rows, **one)
         assert lib.gcn_logits_process(ctypes.byref(d), None, None, None) == rc, rows
         assert lib.gcn_logits_process_bwd(ctypes.byref(d), None, None, None, None, None, 0, None) == rc, rows
+
+
+@pytest.mark.parametrize("name", ["repetition_penalty", "presence_penalty", "frequency_penalty", "temperature"])
+def test_numbers_that_are_not_finite_in_float32_are_refused(name):
+    """1e39 is a finite double and an infinite float; the reciprocal of 1e-39 is infinite, and makes NaN of a logit of 0."""
+    for value in (1e39, -1e39) + ((1e-39,) if name in ("repetition_penalty", "temperature") else ()):
+        with pytest.raises(ValueError):
+            process_logits(X, **{name: value})
+    with pytest.raises(L.GcnHipError, match="no CPU fallback"):              # allowed
+        process_logits(X, **{name: 1e-37})
+
+
+def test_c_entry_points_refuse_numbers_that_are_not_finite():
+    lib = L.load()
+    ok = dict(rows=4, vocab=8, inner=1, in_stride=8, out_stride=8, repetition=1.0, temperature=1.0)
+    for bad in (dict(repetition=math.inf), dict(repetition=1e-39), dict(temperature=math.inf), dict(temperature=1e-39), dict(presence=math.nan),
+                dict(presence=math.inf), dict(frequency=-math.inf)):
+        d = L.LogitsDesc(**{**ok, **bad})
+        assert lib.gcn_logits_process(ctypes.byref(d), None, None, None) == -1 and b"null pointer" not in lib.gcn_last_error(), bad
