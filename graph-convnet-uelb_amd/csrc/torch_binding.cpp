@@ -18,6 +18,7 @@
 #include <optional>
 #include <sstream>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/gcn_uelb_hip.h"
@@ -163,12 +164,16 @@ void adamw_step(py::handle params_, py::handle grads_, py::handle exp_avgs_, py:
     const c10::Device d = params.t[0]->device();
     need_gpu(*params.t[0], "tensor");
     for (List* l : {&params, &grads, &m, &v, &masters, &em, &ev}) l->place(d, l != &grads);
-    // a tensor twice would be updated by two workgroups at once
-    std::vector<void*> once;
+    // a tensor twice, or a part of another, would be updated by two workgroups at once
+    const size_t width = half ? 2 : 4;
+    std::vector<std::pair<const char*, const char*>> once;
     for (size_t k = 0; k < sizes.size(); ++k)
-        if (sizes[k] > 0) once.push_back(params.ptr[k]);
+        if (sizes[k] > 0) once.emplace_back(static_cast<char*>(params.ptr[k]), static_cast<char*>(params.ptr[k]) + sizes[k] * width);
     std::sort(once.begin(), once.end());
-    if (std::adjacent_find(once.begin(), once.end()) != once.end()) value_error("a parameter is in the list twice");
+    for (size_t k = 1; k < once.size(); ++k) {
+        if (once[k].first == once[k - 1].first) value_error("a parameter is in the list twice");
+        if (once[k].first < once[k - 1].second) value_error("parameters overlap in memory");
+    }
     const void* hyper = nullptr;
     if (!hyper_.is_none()) {
         const at::Tensor* t = as_tensor(hyper_);

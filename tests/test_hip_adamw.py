@@ -581,3 +581,19 @@ def test_autograd_hears_of_the_update(dev, A):
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_parameters_that_overlap_are_refused(dev, A):
+    """One that starts inside another; neighbours in one buffer are allowed."""
+    buffer = torch.ones(40, device=dev)
+
+    def step(a, b):
+        state = [[torch.zeros_like(x) for x in (a, b)] for _ in range(2)]
+        A.adamw_step_([a, b], [torch.ones_like(a), torch.ones_like(b)], *state, step=1, lr=1e-2)
+    with pytest.raises(ValueError, match="overlap"):
+        step(buffer[:20], buffer[19:])
+    with pytest.raises(ValueError, match="twice"):
+        step(buffer[:20], buffer[:30])
+    assert torch.equal(buffer, torch.ones_like(buffer))
+    step(buffer[20:], buffer[:20])
+    assert bool((buffer < 1).all())
