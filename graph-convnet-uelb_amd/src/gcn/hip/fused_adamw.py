@@ -234,6 +234,9 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         L.load()
         jobs = self._collect()
+        # before anything is counted
+        if jobs and not self.capturable and torch.cuda.is_current_stream_capturing():
+            raise L.GcnHipError("FusedAdamW: a captured step would repeat its step count: pass capturable=True")
         max_norm = self.max_grad_norm if max_grad_norm is None else max_grad_norm
         coef = self._clip(jobs, max_norm, grad_scale) if max_norm is not None and jobs else None
         advanced = {}

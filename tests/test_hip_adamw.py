@@ -597,3 +597,17 @@ def test_parameters_that_overlap_are_refused(dev, A):
     assert torch.equal(buffer, torch.ones_like(buffer))
     step(buffer[20:], buffer[:20])
     assert bool((buffer < 1).all())
+
+
+def test_a_refused_capture_counts_no_step(dev, A):
+    p = torch.nn.Parameter(torch.ones(8, device=dev))
+    p.grad = torch.ones_like(p)
+    opt = A.FusedAdamW([p])
+    opt.step()
+    before = p.detach().clone()
+    with pytest.raises(RuntimeError, match="capturable"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert float(opt.state[p]["step"]) == 1 and torch.equal(p.detach(), before)
+    opt.step()
+    assert float(opt.state[p]["step"]) == 2
