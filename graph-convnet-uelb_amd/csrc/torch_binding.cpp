@@ -298,6 +298,18 @@ at::Tensor run_forward(Rules& r, const at::Tensor& x, const at::Tensor& out) {
     return out;
 }
 
+// A leaf's gradients are accumulated by a node that lives as long as any graph over the leaf does, on the stream of the first of
+// them.  A captured backward that meets one of another stream would wait for work outside its capture, which ends the process.
+void check_leaf(const at::Tensor& t, const char* name) {
+    if (!t.requires_grad() || !t.is_leaf()) return;
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) return;
+    const std::optional<c10::Stream> stream = node->stream();
+    if (stream && *stream != c10::hip::getCurrentHIPStream(t.device().index()).unwrap())
+        gcn_error("process_logits: ", name, " is a leaf of a graph that lives on another stream; free what that graph computed (its outputs) "
+                  "before capturing one, or capture over a detached copy");
+}
+
 struct ProcessLogits : torch::autograd::Function<ProcessLogits> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const std::optional<at::Tensor>& bias, const at::Tensor& x,
                               c10::intrusive_ptr<Rules> r) {
@@ -425,6 +437,13 @@ py::object process_logits(py::handle logits_, int64_t dim, py::handle history_, 
     if (d.in_stride < 0) {
         x = logits.detach().contiguous();
         d.in_stride = d.vocab * d.inner;
+    }
+    if (grad) {
+        c10::DeviceGuard guard(logits.device());
+        if (capturing()) {
+            check_leaf(logits, "logits");
+            if (bias) check_leaf(*bias, "bias");
+        }
     }
     if (grad) return py::cast(ProcessLogits::apply(logits, bias ? std::optional<at::Tensor>(*bias) : std::nullopt, x.detach(), rules));
     if (out) {

@@ -364,3 +364,27 @@ def test_more_workgroups_than_one_grid_dimension(dev):
     assert torch.equal(y, (x + bias) * 2)
     dx, db = torch.autograd.grad(y, [z, b], torch.ones_like(y))
     assert bool((dx == 2).all()) and bool((db == 2).all())
+
+
+def test_capture_over_a_leaf_of_a_living_graph_is_refused(dev):
+    """The refusal comes before anything is recorded; once the eager graph is gone, the capture works."""
+    from src.gcn.hip.logits import process_logits
+    x = torch.randn(4, 100, device=dev).requires_grad_()
+    bias = torch.randn(100, device=dev).requires_grad_()
+    for kept in (lambda: process_logits(x, temperature=2.0), lambda: bias * 2):
+        alive = kept()
+        with pytest.raises(RuntimeError, match="leaf of a graph that lives"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                process_logits(x, bias=bias)
+        with torch.no_grad():                                # no gradient, no refusal
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                process_logits(x, bias=bias)
+        del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx, = torch.autograd.grad(process_logits(x, bias=bias, temperature=2.0), [x], torch.ones(4, 100, device=dev))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((dx == 0.5).all())
+        dx.zero_()
