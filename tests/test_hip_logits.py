@@ -388,3 +388,42 @@ def test_capture_over_a_leaf_of_a_living_graph_is_refused(dev):
         torch.cuda.synchronize()
         assert bool((dx == 0.5).all())
         dx.zero_()
+
+
+@pytest.mark.parametrize("wide", [torch.int32, torch.int64])
+@pytest.mark.parametrize("inner", [1, 3])
+def test_entries_that_equal_a_place_modulo_2_to_the_32_are_skipped(dev, wide, inner):
+    """Padding of any kind, in forward and backward: negative entries, the type's ends, and in 64 bits those that differ from a place
+    by a multiple of 2^32 or 2^31.  Histories shorter and longer than a turn of the walk, with prompts of every kind."""
+    from src.gcn.hip.logits import process_logits
+    vocab = 9000
+    pads = [-1, -vocab, vocab, 2 ** 31 - 1, -2 ** 31, vocab + 4096]
+    if wide == torch.int64:
+        pads += [2 ** 32 + 5, 2 ** 31 + 5, -2 ** 32 + 5, 2 ** 40 + 5, 2 ** 63 - 1, -2 ** 63, 2 ** 32 + 5000, -2 ** 32 + 8999]
+    gen = torch.Generator().manual_seed(4)
+    for length in (40, 2500, 9000):
+        real = torch.randint(0, vocab, (2, length), generator=gen)
+        keep = torch.rand(2, length, generator=gen) < 0.5
+        padded = torch.where(keep, real, torch.tensor(pads)[torch.randint(0, len(pads), (2, length), generator=gen)]).to(wide)
+        # the same entries without padding: those that count, in place; the rest become one entry outside
+        plain = torch.where(keep, real, -1).to(wide)
+        prompt = torch.tensor([length // 3, -5], dtype=wide, device=dev)
+        shape = (2, vocab) if inner == 1 else (2, vocab, inner)
+        x = torch.randn(shape, generator=gen).to(dev).requires_grad_()
+        kind = dict(dim=1, repetition_penalty=1.5, presence_penalty=0.5, frequency_penalty=0.25, prompt_lens=prompt)
+        got, want = (process_logits(x, history=h.to(dev), **kind) for h in (padded, plain))
+        assert torch.equal(got, want)
+        counts = torch.zeros(2, vocab, dtype=torch.float64)
+        seen = torch.zeros(2, vocab, dtype=torch.bool)
+        for r in range(2):
+            first = max(0, int(prompt[r]))
+            counts[r] = torch.bincount(real[r, first:][keep[r, first:]], minlength=vocab).double()
+            seen[r] = torch.bincount(real[r][keep[r]], minlength=vocab) > 0
+        z = x.detach().cpu().double().view(2, vocab, inner)
+        slope = torch.where(seen.unsqueeze(-1), torch.where(z > 0, 1 / 1.5, 1.5), 1.0)
+        y = z * slope - (counts * 0.25 + (counts > 0) * 0.5).unsqueeze(-1)
+        # 1 / 1.5 and the product, the two terms' sum and the difference: four roundings of at most 2^-24 of what they round
+        bound = 4 * 2.0 ** -24 * ((z * slope).abs() + (counts * 0.25 + 0.5).unsqueeze(-1)) + 1e-37
+        assert bool(((got.detach().cpu().double().view(2, vocab, inner) - y).abs() <= bound).all())
+        dx, = torch.autograd.grad(got, [x], torch.ones_like(got))
+        assert bool(((dx.cpu().double().view(2, vocab, inner) - slope).abs() <= 2.0 ** -23 * slope).all())
