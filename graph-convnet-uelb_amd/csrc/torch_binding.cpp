@@ -250,14 +250,17 @@ struct Rules : torch::CustomClassHolder {
     at::Tensor bias;
 
     // rows of an argument whose leading dimensions are the first `lead` of t: all of the logits' leading dimensions, the last few
-    // of them, or ones
+    // of them, or ones.  The outermost that it has may divide the logits' own: their row o takes row o mod rows
     long long rows_of(const char* name, const at::Tensor& t, int64_t lead, const at::Tensor& logits) const {
         int64_t n = 1, skip = 0;
         for (int64_t k = 0; k < lead; ++k) n *= t.size(k);
         if (n == 1) return 1;
         while (lead - skip > dim && t.size(skip) == 1) ++skip;
         bool fits = lead - skip <= dim;
-        for (int64_t k = skip; fits && k < lead; ++k) fits = t.size(k) == logits.size(dim - lead + k);
+        for (int64_t k = skip; fits && k < lead; ++k) {
+            const int64_t have = t.size(k), of = logits.size(dim - lead + k);
+            fits = have == of || (k == skip && have > 0 && of % have == 0);
+        }
         if (!fits) value_error(name, ": leading dimensions ", t.sizes().slice(0, lead), " do not match the logits' ", logits.sizes().slice(0, dim), " from the last one on");
         return n;
     }

@@ -29,7 +29,9 @@ def process_logits(logits, *, dim=-1, history=None, history_lens=None, prompt_le
     """The logits after penalties, bias, temperature and mask, of the same shape and type.
 
     logits: float32, bfloat16 or float16 ``[*lead, V, *inner]`` with the vocabulary at ``dim``.  The other arguments hold rows
-    for ``lead``, for its last few dimensions (the same for all others), or one row for all, and apply to all of ``inner``:
+    for ``lead``, for its last few dimensions (the same for all others), or one row for all, and apply to all of ``inner``.  The
+    outermost dimension of their rows may also be a divisor of the logits' own there: R rows for N = k R rows of logits,
+    whose row o uses row o mod R, as link scores [graphs * V, V, C] use a bias [V, V] of the node.
       history ``[*rows, length]``, int32 or int64: entries that occurred; those outside ``[0, V)`` are skipped (padding).
         history_lens, prompt_lens ``[*rows]``: the first history_lens entries count; those before prompt_lens count for the
         repetition penalty only.  The same entry may occur any number of times.

@@ -427,3 +427,19 @@ def test_entries_that_equal_a_place_modulo_2_to_the_32_are_skipped(dev, wide, in
         assert bool(((got.detach().cpu().double().view(2, vocab, inner) - y).abs() <= bound).all())
         dx, = torch.autograd.grad(got, [x], torch.ones_like(got))
         assert bool(((dx.cpu().double().view(2, vocab, inner) - slope).abs() <= 2.0 ** -23 * slope).all())
+
+
+@pytest.mark.parametrize("rows, vocab, inner, period", [(12, 6, 10, 6), (28, 14, 5, 14), (30, 100, 1, 5), (6, 2049, 1, 2), (7, 9, 3, 1), (8, 8, 4, 8)])
+def test_flat_rows_take_the_rows_of_an_argument_in_turn(dev, rows, vocab, inner, period):
+    """Logits with one leading dimension and arguments with a divisor of it: row o uses row o mod R, with its gradient."""
+    x, kind, want = case(dev, rows, vocab, inner, seed=period, bias_rows=period, hist_rows=period)
+    lead = x.dim() - (1 if inner == 1 else 2)
+    flat = {k: v.flatten(0, lead - 1) if isinstance(v, torch.Tensor) and v.dim() > 1 and v.shape[:lead] == x.shape[:lead] else v for k, v in kind.items()}
+    flat = {**flat, "dim": 1, **{k: flat[k].reshape(rows) for k in ("repetition_penalty", "presence_penalty", "frequency_penalty", "temperature")}}
+    assert flat["bias"].shape == (period, vocab) and flat["history"].shape[0] == period and flat["mask"].shape[0] == rows
+    z = x.reshape(rows, vocab) if inner == 1 else x.reshape(rows, vocab, inner)
+    check(z, flat, want)
+    dy = torch.randn(z.shape, device=dev, generator=torch.Generator(dev).manual_seed(2))
+    got = grads(z, flat, want, period, dy)
+    base = grads(x, kind, want, period, dy.view(x.shape))
+    assert torch.equal(got[0].view(x.shape), base[0]) and torch.equal(got[1], base[1])

@@ -160,3 +160,16 @@ def test_c_entry_points_refuse_numbers_that_are_not_finite():
                 dict(presence=math.inf), dict(frequency=-math.inf)):
         d = L.LogitsDesc(**{**ok, **bad})
         assert lib.gcn_logits_process(ctypes.byref(d), None, None, None) == -1 and b"null pointer" not in lib.gcn_last_error(), bad
+
+
+@pytest.mark.parametrize("lead, rows, fits", [
+    ((6,), (6,), True), ((6,), (3,), True), ((6,), (2,), True), ((6,), (1,), True), ((6,), (4,), False), ((6,), (12,), False), ((6,), (0,), False),
+    ((4, 3), (4, 3), True), ((4, 3), (3,), True), ((4, 3), (2, 3), True), ((4, 3), (1, 3), True), ((4, 3), (4, 1), False), ((4, 3), (3, 3), False),
+    ((4, 6), (3,), True), ((4, 6), (2, 3), False), ((4, 6), (4,), False), ((6,), (1, 3), True), ((), (2,), False), ((), (1,), True)])
+def test_rows_of_an_argument(lead, rows, fits):
+    """All leading dimensions, the last few, one row, or a divisor at the outermost; what fits is refused for being on the CPU."""
+    x = torch.zeros(*lead, 10)
+    for kind in (dict(bias=torch.zeros(*rows, 10)), dict(mask=torch.ones(*rows, 10, dtype=torch.bool)), dict(temperature=torch.ones(*rows)),
+                 dict(history=torch.zeros(*rows, 4, dtype=torch.int64))):
+        with pytest.raises(L.GcnHipError if fits else ValueError, match="no CPU fallback" if fits else "leading dimensions"):
+            process_logits(x, **kind)
