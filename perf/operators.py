@@ -153,9 +153,7 @@ def _prepare_logits(c, seed):
     rows, vocab, inner, length, kind = c["rows"], c["vocab"], c["inner"], c["history"], TYPES[c["type"]]
     rand = lambda *n: torch.rand(*n, device=dev, generator=gen)  # noqa: E731
     logits = 3 * torch.randn(rows, vocab, inner, device=dev, generator=gen)
-    # one row for each request or position; with a bias of every node, rows of (graph, node)
-    lead = (rows // vocab, vocab) if c["bias"] == "period" else (rows,)
-    s = {"case": c, "dim": len(lead), "masked": -1e9 if inner > 1 else -math.inf}
+    s = {"case": c, "masked": -1e9 if inner > 1 else -math.inf}
     if inner == 1:
         # common tokens come often; requests have contexts of their own lengths, a quarter of each is the prompt
         s["history"] = (vocab * rand(rows, length) ** 4).long().clamp_(0, vocab - 1)
@@ -168,11 +166,10 @@ def _prepare_logits(c, seed):
         s["history"] = torch.where(rand(rows, length) < 0.3, (vocab * rand(rows, length)).long().clamp_(0, vocab - 1), -1)
         s["lens"] = s["prompts"] = None
         s["repetition"], s["presence"], s["frequency"], s["temperature"] = 1.2, 0.1, 0.25, 0.9
-    logits = logits.to(kind).view((*lead, vocab) if inner == 1 else (*lead, vocab, inner))
+    logits = logits.to(kind).view((rows, vocab) if inner == 1 else (rows, vocab, inner))
     if c["pad"]:
-        logits = torch.nn.functional.pad(logits, (0, c["pad"]))[..., :vocab]
+        logits = torch.nn.functional.pad(logits, (0, c["pad"]))[:, :vocab]
     s["logits"] = logits
-    s |= {k: v.view(*lead, *v.shape[1:]) for k, v in s.items() if k not in ("case", "logits") and isinstance(v, torch.Tensor)}
     bias_rows = {"none": 0, "shared": 1, "period": vocab, "rows": rows}[c["bias"]]
     s["bias"] = torch.randn(bias_rows, vocab, device=dev, generator=gen) if bias_rows else None
     s["mask"] = None
@@ -182,7 +179,6 @@ def _prepare_logits(c, seed):
         share = torch.where(rand(rows, 1) < 1 / 16, torch.zeros_like(share), share)
         allowed = rand(rows, vocab) < share
         s["mask"] = allowed if c["mask"] == "bool" else _bits_of(allowed)
-        s["mask"] = s["mask"].view(*lead, -1)
     s["grad"] = torch.randn(rows, vocab, inner, device=dev, generator=gen).to(kind).view(logits.shape) * 2.0 ** -8 if c["train"] else None
     return s
 
@@ -310,7 +306,7 @@ def _plain_adamw(s):
 
 def _own_logits(s):
     _, logits = _package()
-    rules = dict(dim=s["dim"], history=s["history"], history_lens=s["lens"], prompt_lens=s["prompts"], repetition_penalty=s["repetition"],
+    rules = dict(dim=1, history=s["history"], history_lens=s["lens"], prompt_lens=s["prompts"], repetition_penalty=s["repetition"],
                  presence_penalty=s["presence"], frequency_penalty=s["frequency"], mask=s["mask"], temperature=s["temperature"], masked_value=s["masked"])
     if s["grad"] is None:
         return logits.process_logits(s["logits"], bias=s["bias"], **rules)
@@ -326,8 +322,7 @@ def _column(value):
 
 def _counts(s, rows, vocab):
     """How often each token stands in each row's history: anywhere, and behind the prompt."""
-    ids = s["history"].view(rows, -1)
-    place = torch.arange(ids.shape[1], device=ids.device)
+    ids, place = s["history"], torch.arange(s["history"].shape[1], device=s["history"].device)
     valid = (ids >= 0) & (ids < vocab)
     valid = valid if s["lens"] is None else valid & (place < s["lens"].view(-1, 1))
     after = valid if s["prompts"] is None else valid & (place >= s["prompts"].view(-1, 1))
@@ -338,7 +333,7 @@ def _counts(s, rows, vocab):
 def _plain_logits(s):
     c = s["case"]
     rows, vocab, inner = c["rows"], c["vocab"], c["inner"]
-    x = s["logits"].reshape(rows, vocab, inner).float()
+    x = s["logits"].view(rows, vocab, -1).float() if inner == 1 else s["logits"].float()
     rho, tau = _column(s["repetition"]), _column(s["temperature"])
     every, new = _counts(s, rows, vocab)
     seen, up = every > 0, x > 0
@@ -347,7 +342,7 @@ def _plain_logits(s):
     if s["bias"] is not None:
         y = y + s["bias"].repeat(rows // s["bias"].shape[0], 1).unsqueeze(2)
     y = y / tau
-    allowed = None if s["mask"] is None else _truth_of(s["mask"].view(rows, -1), vocab).unsqueeze(2)
+    allowed = None if s["mask"] is None else _truth_of(s["mask"], vocab).unsqueeze(2)
     if allowed is not None:
         y = torch.where(allowed, y, s["masked"])
     y = y.to(s["logits"].dtype).view(s["logits"].shape)
@@ -425,10 +420,10 @@ def _exact_logits(c, seed):
     x = s["logits"].double().reshape(rows, vocab, inner)
     number = lambda v: v.double().view(-1, 1, 1) if isinstance(v, torch.Tensor) else v  # noqa: E731
     rho, tau = number(s["repetition"]), number(s["temperature"])
-    ids, length = s["history"].view(rows, -1), c["history"]
+    ids, length = s["history"], c["history"]
     place = torch.arange(length, device=ids.device).expand(rows, length)
-    used = ids >= 0 if s["lens"] is None else place < s["lens"].view(-1, 1)
-    after = used if s["prompts"] is None else used & (place >= s["prompts"].view(-1, 1))
+    used = ids >= 0 if s["lens"] is None else place < s["lens"].unsqueeze(1)
+    after = used if s["prompts"] is None else used & (place >= s["prompts"].unsqueeze(1))
     cell = ids + vocab * torch.arange(rows, device=ids.device).unsqueeze(1)
     seen = torch.bincount(cell[used], minlength=rows * vocab).view(rows, vocab, 1) > 0
     new = torch.bincount(cell[after], minlength=rows * vocab).view(rows, vocab, 1)
@@ -437,7 +432,7 @@ def _exact_logits(c, seed):
     y -= (number(s["frequency"]) * new + number(s["presence"]) * (new > 0).double()) / tau
     if s["bias"] is not None:
         y += (s["bias"].double().repeat(rows // s["bias"].shape[0], 1).unsqueeze(2)) / tau
-    off = torch.zeros(rows, vocab, 1, dtype=torch.bool, device=x.device) if s["mask"] is None else ~_truth_of(s["mask"].view(rows, -1), vocab).unsqueeze(2)
+    off = torch.zeros(rows, vocab, 1, dtype=torch.bool, device=x.device) if s["mask"] is None else ~_truth_of(s["mask"], vocab).unsqueeze(2)
     y = y.masked_fill(off, s["masked"]).view(s["logits"].shape)
     if s["grad"] is None:
         return y
