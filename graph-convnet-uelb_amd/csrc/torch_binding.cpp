@@ -15,6 +15,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
+#include <cstring>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -243,10 +245,28 @@ int64_t row_stride(const at::Tensor& t, int64_t dim) {
     return stride < 0 ? want : stride;
 }
 
+// What a tensor that is saved for the backward pass has to be when it comes back: hooks on saved tensors may return another one,
+// with strides and an address of its own.
+struct Saved {
+    const char* name;
+    std::vector<int64_t> sizes;
+    at::ScalarType type;
+    c10::Device device;
+
+    Saved(const char* name, const at::Tensor& t) : name(name), sizes(t.sizes().vec()), type(t.scalar_type()), device(t.device()) {}
+    void check(const at::Tensor& t) const {
+        TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.sizes() == at::IntArrayRef(sizes) && t.scalar_type() == type && t.device() == device,
+                    "process_logits: ", name, " was saved as ", type, " ", at::IntArrayRef(sizes), " on ", device, " and came back as something else");
+    }
+};
+
 struct Rules : torch::CustomClassHolder {
     gcn_logits_desc d = {};
     int64_t dim = 0;
-    std::vector<at::Tensor> kept;                  // what the descriptor points into (the bias apart)
+    std::vector<at::Tensor> kept;                  // what the descriptor points into (the bias apart), until it is saved
+    std::vector<size_t> fields;                    // which of its fields, as offsets
+    std::vector<const char*> names;
+    std::vector<Saved> saved;                      // the logits, then what was kept
     at::Tensor bias;
 
     // rows of an argument whose leading dimensions are the first `lead` of t: all of the logits' leading dimensions, the last few
@@ -264,10 +284,50 @@ struct Rules : torch::CustomClassHolder {
         if (!fits) value_error(name, ": leading dimensions ", t.sizes().slice(0, lead), " do not match the logits' ", logits.sizes().slice(0, dim), " from the last one on");
         return n;
     }
-    const void* place(const char* name, const at::Tensor& t, const at::Tensor& logits) {
+    // t's address goes into the descriptor's field at that offset (a pointer to const); t is made contiguous
+    static void point(gcn_logits_desc* d, size_t field, const at::Tensor& t) {
+        const void* address = t.const_data_ptr();
+        std::memcpy(reinterpret_cast<char*>(d) + field, &address, sizeof(address));
+    }
+    void place(const char* name, const at::Tensor& t, const at::Tensor& logits, size_t field) {
         if (t.device() != logits.device()) value_error(name, " is on ", t.device(), ", the logits are on ", logits.device());
         kept.push_back(t.is_contiguous() ? t : t.contiguous());
-        return kept.back().const_data_ptr();
+        fields.push_back(field);
+        names.push_back(name);
+        point(&d, field, kept.back());
+    }
+    // What the gradient reads (not the bias): the logits, then what was kept.  From here on only autograd holds it, and its own
+    // check of changes in between covers it.
+    std::vector<at::Tensor> save(const at::Tensor& x) {
+        std::vector<at::Tensor> out{x};
+        saved.emplace_back("logits", x);
+        for (size_t k = 0; k < kept.size(); ++k) {
+            saved.emplace_back(names[k], kept[k]);
+            out.push_back(std::move(kept[k]));
+        }
+        kept.clear();
+        return out;
+    }
+    // The descriptor for what came back; `back` keeps what it points into, the logits first.
+    gcn_logits_desc restore(std::vector<at::Tensor>* back) const {
+        TORCH_CHECK(back->size() == saved.size(), "process_logits: saved tensors are missing");
+        for (size_t k = 0; k < back->size(); ++k) saved[k].check((*back)[k]);
+        gcn_logits_desc now = d;
+        at::Tensor& x = (*back)[0];
+        now.in_stride = row_stride(x, dim);
+        if (now.in_stride < 0) {
+            x = x.contiguous();
+            now.in_stride = now.vocab * now.inner;
+        }
+        for (size_t k = 0; k < fields.size(); ++k) {
+            const void* was;
+            std::memcpy(&was, reinterpret_cast<const char*>(&d) + fields[k], sizeof(was));
+            if (!was) continue;                     // not used: lengths of an empty history
+            at::Tensor& t = (*back)[k + 1];
+            if (!t.is_contiguous()) t = t.contiguous();
+            point(&now, fields[k], t);
+        }
+        return now;
     }
 };
 
@@ -280,12 +340,12 @@ const at::Tensor* tensor_or_none(py::handle h, const char* name) {
     return t;
 }
 
-void penalty(Rules& r, py::handle h, const char* name, const at::Tensor& logits, bool positive, float* value, const float** table, long long* rows) {
+void penalty(Rules& r, py::handle h, const char* name, const at::Tensor& logits, bool positive, float* value, size_t table, long long* rows) {
     *rows = 1;
     if (const at::Tensor* t = as_tensor(h)) {
         if (t->scalar_type() != at::kFloat) type_error(name, " is a number or float32, got ", t->scalar_type());
         *rows = r.rows_of(name, *t, t->dim(), logits);
-        *table = static_cast<const float*>(r.place(name, *t, logits));
+        r.place(name, *t, logits, table);
         return;
     }
     const double x = PyFloat_AsDouble(h.ptr());
@@ -318,22 +378,20 @@ struct ProcessLogits : torch::autograd::Function<ProcessLogits> {
                               c10::intrusive_ptr<Rules> r) {
         at::Tensor out = at::empty(logits.sizes(), logits.options());
         if (logits.numel()) run_forward(*r, x, out);
-        // what the gradient reads (not the bias) is saved, for autograd's own check of changes in between
-        std::vector<at::Tensor> saved{x};
-        saved.insert(saved.end(), r->kept.begin(), r->kept.end());
-        ctx->save_for_backward(saved);
+        ctx->save_for_backward(r->save(x));
         ctx->saved_data["rules"] = c10::IValue::make_capsule(r);
         if (bias) ctx->saved_data["bias_shape"] = bias->sizes().vec();
         return out;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-        const at::Tensor x = ctx->get_saved_variables()[0];
+        std::vector<at::Tensor> back = ctx->get_saved_variables();
         const bool want_x = ctx->needs_input_grad(0), want_bias = ctx->saved_data.count("bias_shape") && ctx->needs_input_grad(1);
         at::Tensor dx, dbias;
         {
             at::NoGradGuard no_grad;
             c10::intrusive_ptr<torch::CustomClassHolder> holder = ctx->saved_data["rules"].toCapsule();
-            gcn_logits_desc d = static_cast<Rules*>(holder.get())->d;
+            gcn_logits_desc d = static_cast<Rules*>(holder.get())->restore(&back);
+            const at::Tensor& x = back[0];
             const at::Tensor dy = grads[0].contiguous();
             d.out_stride = d.vocab * d.inner;
             c10::DeviceGuard guard(x.device());
@@ -389,30 +447,30 @@ py::object process_logits(py::handle logits_, int64_t dim, py::handle history_, 
         d.history_rows = r.rows_of("history", *history, history->dim() - 1, logits);
         d.history_len = history->size(-1);
         d.history_wide = history->scalar_type() == at::kLong;
-        d.history = r.place("history", *history, logits);
+        r.place("history", *history, logits, offsetof(gcn_logits_desc, history));
         for (const at::Tensor* t : {lens, prompts}) {
             if (!t) continue;
             if (!is_int(*t) || (lens && t->scalar_type() != lens->scalar_type())) type_error("history_lens and prompt_lens are int32 or int64, both alike");
             if (t->sizes() != history->sizes().slice(0, history->dim() - 1))
                 value_error("lengths of shape ", t->sizes(), " for a history with rows ", history->sizes().slice(0, history->dim() - 1));
             d.lens_wide = t->scalar_type() == at::kLong;
-            (t == lens ? d.history_lens : d.prompt_lens) = r.place("history_lens and prompt_lens", *t, logits);
+            r.place("history_lens and prompt_lens", *t, logits, t == lens ? offsetof(gcn_logits_desc, history_lens) : offsetof(gcn_logits_desc, prompt_lens));
         }
         // without entries nothing is read; an empty tensor has no address
         if (!d.history) d.history_lens = d.prompt_lens = nullptr;
     } else if (lens || prompts) {
         value_error("history_lens and prompt_lens go with a history");
     }
-    penalty(r, repetition, "repetition penalty", logits, true, &d.repetition, &d.repetition_t, &d.repetition_rows);
-    penalty(r, presence, "presence penalty", logits, false, &d.presence, &d.presence_t, &d.presence_rows);
-    penalty(r, frequency, "frequency penalty", logits, false, &d.frequency, &d.frequency_t, &d.frequency_rows);
-    penalty(r, temperature, "temperature", logits, true, &d.temperature, &d.temperature_t, &d.temperature_rows);
+    penalty(r, repetition, "repetition penalty", logits, true, &d.repetition, offsetof(gcn_logits_desc, repetition_t), &d.repetition_rows);
+    penalty(r, presence, "presence penalty", logits, false, &d.presence, offsetof(gcn_logits_desc, presence_t), &d.presence_rows);
+    penalty(r, frequency, "frequency penalty", logits, false, &d.frequency, offsetof(gcn_logits_desc, frequency_t), &d.frequency_rows);
+    penalty(r, temperature, "temperature", logits, true, &d.temperature, offsetof(gcn_logits_desc, temperature_t), &d.temperature_rows);
     if (const at::Tensor* mask = tensor_or_none(mask_, "mask")) {
         if ((mask->scalar_type() != at::kBool && mask->scalar_type() != at::kInt) || mask->dim() == 0) type_error("mask holds truth values, or bits in int32 words");
         d.mask_type = mask->scalar_type() == at::kBool ? 1 : 2;
         if (mask->size(-1) != (d.mask_type == 1 ? d.vocab : (d.vocab + 31) / 32)) value_error("mask of shape ", mask->sizes(), " for ", d.vocab, " entries");
         d.mask_rows = r.rows_of("mask", *mask, mask->dim() - 1, logits);
-        d.mask = r.place("mask", *mask, logits);
+        r.place("mask", *mask, logits, offsetof(gcn_logits_desc, mask));
     }
     const at::Tensor* bias = tensor_or_none(bias_, "bias");
     if (bias) {
@@ -478,4 +536,5 @@ PYBIND11_MODULE(gcn_uelb_torch, m) {
     m.def("grad_norm", &grad_norm);
     m.def("process_logits", &process_logits);
     m.def("row_stride", [](const at::Tensor& t, int64_t dim) { return row_stride(t, dim); });
+    m.def("check_saved", [](const at::Tensor& was, const at::Tensor& now) { Saved("tensor", was).check(now); });
 }

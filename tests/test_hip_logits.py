@@ -443,3 +443,67 @@ def test_flat_rows_take_the_rows_of_an_argument_in_turn(dev, rows, vocab, inner,
     got = grads(z, flat, want, period, dy)
     base = grads(x, kind, want, period, dy.view(x.shape))
     assert torch.equal(got[0].view(x.shape), base[0]) and torch.equal(got[1], base[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("inner", [1, 3])
+def test_saved_tensors_may_come_back_elsewhere(dev, dtype, inner):
+    """Hooks on saved tensors return copies: dense where the logits had padded, expanded or shifted rows, or with other strides."""
+    from src.gcn.hip.logits import process_logits
+    rows, vocab = 7, 37
+    x, kind, _ = case(dev, rows, vocab, inner, length=30, dtype=dtype, seed=5, bias_rows=rows)
+    lead = x.shape[1:]
+    padded = torch.full((rows, vocab + 8, *lead[1:]), 1e3, device=dev, dtype=dtype)
+    padded[:, 3:3 + vocab] = x
+    layouts = {"dense": x, "padded": padded[:, 3:3 + vocab], "expanded": x[:1].expand(rows, *lead),
+               "every other row": torch.stack([x, -x], 1).flatten(0, 1)[::2], "transposed": x.transpose(0, 1).contiguous().transpose(0, 1)}
+
+    def apart(t):                                  # dense rows further apart
+        if t.dim() == 0 or not t.numel():
+            return t.clone()
+        wide = torch.zeros(*t.shape[:1], 2, *t.shape[1:], device=t.device, dtype=t.dtype)
+        wide[:, 1] = t
+        return wide[:, 1]
+
+    turned = lambda t: t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() > 1 else t.clone()
+    same = lambda t: t
+    for name, z in layouts.items():
+        z, b = z.detach().requires_grad_(), kind["bias"].detach().requires_grad_()
+        dy = torch.randn(z.shape, device=dev, generator=torch.Generator(dev).manual_seed(3)).to(dtype)
+        step = lambda: torch.autograd.grad(process_logits(z, **{**kind, "bias": b}, masked_value=-1e4), [z, b], dy)
+        base = step()
+        assert float(base[0].abs().sum()) > 0
+        for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True),
+                      torch.autograd.graph.saved_tensors_hooks(apart, same), torch.autograd.graph.saved_tensors_hooks(same, turned)):
+            with hooks:
+                got = step()
+            assert all(torch.equal(g, w) for g, w in zip(got, base)), (name, hooks)
+        for bad in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t[:1], lambda t: t.unsqueeze(0)):
+            with torch.autograd.graph.saved_tensors_hooks(same, bad):
+                y = process_logits(z, **{**kind, "bias": b}, masked_value=-1e4)
+                with pytest.raises(RuntimeError, match="was saved as"):
+                    torch.autograd.grad(y, [z, b], dy)
+
+
+def test_saved_arguments_are_held_by_autograd_alone(dev):
+    """What a hook moves to the host leaves the GPU: the call keeps no second reference to history and mask."""
+    from src.gcn.hip.logits import process_logits
+    z = torch.randn(4, 1000, device=dev, requires_grad=True)
+    torch.cuda.synchronize()
+    with torch.autograd.graph.save_on_cpu():
+        before = torch.cuda.memory_allocated()
+        y = process_logits(z, history=torch.zeros(4, 1 << 20, dtype=torch.int64, device=dev), repetition_penalty=1.5,
+                           mask=torch.ones(4, 1000, dtype=torch.bool, device=dev))
+        assert torch.cuda.memory_allocated() - before < 1 << 20
+    y.sum().backward()
+    want = torch.ones(4, 1000, device=dev)
+    want[:, 0] = torch.where(z[:, 0] > 0, 1 / torch.tensor(1.5, device=dev), torch.tensor(1.5, device=dev)).detach()
+    assert torch.equal(z.grad, want)
+
+
+def test_lengths_of_an_empty_history_with_gradient(dev):
+    from src.gcn.hip.logits import process_logits
+    z = torch.randn(3, 9, device=dev, requires_grad=True)
+    n = torch.zeros(3, dtype=torch.int64, device=dev)
+    y = process_logits(z, history=torch.zeros(3, 0, dtype=torch.int64, device=dev), history_lens=n, prompt_lens=n, repetition_penalty=2.0)
+    assert torch.equal(torch.autograd.grad(y.sum(), [z])[0], torch.ones_like(z))

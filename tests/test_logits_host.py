@@ -173,3 +173,14 @@ def test_rows_of_an_argument(lead, rows, fits):
                  dict(history=torch.zeros(*rows, 4, dtype=torch.int64))):
         with pytest.raises(L.GcnHipError if fits else ValueError, match="no CPU fallback" if fits else "leading dimensions"):
             process_logits(x, **kind)
+
+
+def test_a_saved_tensor_comes_back_as_what_it_was():
+    """Hooks on saved tensors may change strides and addresses, and nothing else."""
+    same = L.binding().check_saved
+    x = torch.zeros(3, 10, dtype=torch.bfloat16)
+    for now in (x, x.clone(), torch.zeros(10, 3, dtype=torch.bfloat16).t(), torch.zeros(3, 16, dtype=torch.bfloat16)[:, :10]):
+        same(x, now)
+    for now in (x.float(), x.half(), x[:2], x[:, :9], x.view(30), x.view(1, 3, 10), x.to("meta"), x.to_sparse()):
+        with pytest.raises(RuntimeError, match="was saved as"):
+            same(x, now)
