@@ -373,6 +373,11 @@ void check_leaf(const at::Tensor& t, const char* name) {
                   "before capturing one, or capture over a detached copy");
 }
 
+// There is no forward-mode derivative: a tangent would be lost without a word.
+void check_tangent(const at::Tensor& t, const char* name) {
+    if (t._fw_grad(0).defined()) gcn_error("process_logits: ", name, " carries a tangent, and there is no forward-mode derivative");
+}
+
 struct ProcessLogits : torch::autograd::Function<ProcessLogits> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const std::optional<at::Tensor>& bias, const at::Tensor& x,
                               c10::intrusive_ptr<Rules> r) {
@@ -429,6 +434,7 @@ py::object process_logits(py::handle logits_, int64_t dim, py::handle history_, 
     const at::Tensor* lp = as_tensor(logits_);
     if (!lp || type_id(lp->scalar_type()) < 0) type_error("logits are float32, bfloat16 or float16 tensors");
     const at::Tensor& logits = *lp;
+    check_tangent(logits, "logits");
     if (dim < -logits.dim() || dim >= logits.dim()) value_error("logits of shape ", logits.sizes(), " have no dimension ", dim);
     auto rules = c10::make_intrusive<Rules>();
     Rules& r = *rules;
@@ -474,6 +480,7 @@ py::object process_logits(py::handle logits_, int64_t dim, py::handle history_, 
     }
     const at::Tensor* bias = tensor_or_none(bias_, "bias");
     if (bias) {
+        check_tangent(*bias, "bias");
         if (bias->scalar_type() != at::kFloat || bias->dim() == 0) type_error("bias is float32 [..., vocabulary]");
         if (bias->size(-1) != d.vocab) value_error("bias of shape ", bias->sizes(), " for ", d.vocab, " entries");
         d.bias_rows = r.rows_of("bias", *bias, bias->dim() - 1, logits);
@@ -484,6 +491,7 @@ py::object process_logits(py::handle logits_, int64_t dim, py::handle history_, 
     const bool grad = at::GradMode::is_enabled() && (logits.requires_grad() || (bias && bias->requires_grad()));
     const at::Tensor* out = tensor_or_none(out_, "out");
     if (out) {
+        check_tangent(*out, "out");
         if (grad || (at::GradMode::is_enabled() && out->requires_grad())) value_error("out does not go with gradients");
         if (out->sizes() != logits.sizes() || out->scalar_type() != logits.scalar_type() || out->device() != logits.device())
             value_error("out is a tensor like the logits");

@@ -41,7 +41,8 @@ def process_logits(logits, *, dim=-1, history=None, history_lens=None, prompt_le
       mask: what is allowed, as truth values ``[*rows, V]`` or as bits (``pack_mask``); the rest becomes masked_value (rounded
         to the logits' type: -1e9 is -inf in float16).  A row
         whose mask leaves nothing becomes masked_value throughout: with -inf a softmax over it is NaN.
-    Differentiable in logits and bias (at x = 0 with the slope below it); penalties and temperatures are constants.  While a stream
+    Differentiable in logits and bias (at x = 0 with the slope below it); penalties and temperatures are constants.
+    There is no forward-mode derivative: a tangent on logits, bias or out is refused.  While a stream
     is captured, logits and bias that are leaves of a graph which lives on another stream are refused: its backward pass could
     not be captured.
     out: a tensor for the result, which may be ``logits`` and must not overlap it otherwise; not with gradients."""

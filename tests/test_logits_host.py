@@ -184,3 +184,17 @@ def test_a_saved_tensor_comes_back_as_what_it_was():
     for now in (x.float(), x.half(), x[:2], x[:, :9], x.view(30), x.view(1, 3, 10), x.to("meta"), x.to_sparse()):
         with pytest.raises(RuntimeError, match="was saved as"):
             same(x, now)
+
+
+@pytest.mark.parametrize("name", ["logits", "bias", "out"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(name, grad):
+    """No forward-mode derivative: with a tangent the result would be a constant without a word."""
+    import torch.autograd.forward_ad as fwAD
+    given = dict(logits=torch.zeros(3, 10), bias=torch.zeros(10), out=torch.zeros(3, 10))
+    if name != "out":
+        del given["out"]
+    with fwAD.dual_level():
+        given[name] = fwAD.make_dual(given[name].requires_grad_(grad and name != "out"), torch.ones_like(given[name]))
+        with pytest.raises(L.GcnHipError, match=f"{name} carries a tangent"):
+            process_logits(given.pop("logits"), **given)
