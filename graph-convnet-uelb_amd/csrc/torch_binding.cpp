@@ -354,6 +354,42 @@ void penalty(Rules& r, py::handle h, const char* name, const at::Tensor& logits,
     if (!std::isfinite(*value) || (positive && !(*value > 0.f && std::isfinite(1.f / *value)))) value_error(name, " ", x);
 }
 
+// Memory of `rows` rows of `len` bytes, `step` apart.
+struct Region {
+    uintptr_t at;
+    int64_t step, len, rows;
+
+    uintptr_t end() const { return at + (rows - 1) * step + len; }
+    bool meets(uintptr_t lo, uintptr_t hi) const {
+        if (hi <= at || lo >= end()) return false;
+        const int64_t before = static_cast<int64_t>(lo - at) - len;             // the first row that ends behind lo
+        const int64_t k = lo < at || before < 0 ? 0 : before / step + 1;
+        return k < rows && at + k * step < hi;
+    }
+    bool meets(const Region& o) const {
+        if (o.end() <= at || o.at >= end()) return false;
+        for (int64_t k = 0; k < (o.step ? o.rows : 1); ++k)
+            if (meets(o.at + k * o.step, o.at + k * o.step + o.len)) return true;
+        return false;
+    }
+};
+Region region_of(const at::Tensor& t, int64_t stride, int64_t rows) {
+    const int64_t size = t.element_size(), len = t.numel() / rows * size;
+    return {reinterpret_cast<uintptr_t>(t.const_data_ptr()), rows > 1 ? stride * size : len, len, rows};
+}
+// out is written while other workgroups read: its rows are the logits' own, or lie apart from them and from every argument.
+void check_apart(const Rules& r, const at::Tensor& x, const at::Tensor& out) {
+    if (out.numel() == 0) return;
+    const Region to = region_of(out, row_stride(out, r.dim), r.d.rows), from = region_of(x, r.d.in_stride, r.d.rows);
+    if (!(to.at == from.at && to.step == from.step) && to.meets(from)) value_error("out overlaps the logits, and is not the logits themselves");
+    for (size_t k = 0; k <= r.kept.size(); ++k) {
+        const at::Tensor& t = k < r.kept.size() ? r.kept[k] : r.bias;
+        if (!t.defined() || t.numel() == 0) continue;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+        if (to.meets(at, at + t.numel() * t.element_size())) value_error("out overlaps ", k < r.kept.size() ? r.names[k] : "bias");
+    }
+}
+
 at::Tensor run_forward(Rules& r, const at::Tensor& x, const at::Tensor& out) {
     r.d.out_stride = row_stride(out, r.dim);
     c10::DeviceGuard guard(x.device());
@@ -507,6 +543,7 @@ py::object process_logits(py::handle logits_, int64_t dim, py::handle history_, 
         x = logits.detach().contiguous();
         d.in_stride = d.vocab * d.inner;
     }
+    if (out) check_apart(r, x, *out);
     if (grad) {
         c10::DeviceGuard guard(logits.device());
         if (capturing()) {
@@ -544,5 +581,8 @@ PYBIND11_MODULE(gcn_uelb_torch, m) {
     m.def("grad_norm", &grad_norm);
     m.def("process_logits", &process_logits);
     m.def("row_stride", [](const at::Tensor& t, int64_t dim) { return row_stride(t, dim); });
+    m.def("rows_meet", [](const at::Tensor& a, const at::Tensor& b) {
+        return region_of(a, row_stride(a, 1), a.size(0)).meets(region_of(b, row_stride(b, 1), b.size(0)));
+    });
     m.def("check_saved", [](const at::Tensor& was, const at::Tensor& now) { Saved("tensor", was).check(now); });
 }

@@ -45,6 +45,6 @@ def process_logits(logits, *, dim=-1, history=None, history_lens=None, prompt_le
     There is no forward-mode derivative: a tangent on logits, bias or out is refused.  While a stream
     is captured, logits and bias that are leaves of a graph which lives on another stream are refused: its backward pass could
     not be captured.
-    out: a tensor for the result, which may be ``logits`` and must not overlap it otherwise; not with gradients."""
+    out: a tensor for the result, which may be ``logits`` and must not overlap it otherwise, nor any other argument; not with gradients."""
     return L.binding().process_logits(logits, dim, history, history_lens, prompt_lens, repetition_penalty, presence_penalty, frequency_penalty, bias,
                                       mask, temperature, masked_value, out)

@@ -507,3 +507,26 @@ def test_lengths_of_an_empty_history_with_gradient(dev):
     n = torch.zeros(3, dtype=torch.int64, device=dev)
     y = process_logits(z, history=torch.zeros(3, 0, dtype=torch.int64, device=dev), history_lens=n, prompt_lens=n, repetition_penalty=2.0)
     assert torch.equal(torch.autograd.grad(y.sum(), [z])[0], torch.ones_like(z))
+
+
+def test_out_that_overlaps_is_refused(dev):
+    from src.gcn.hip.logits import process_logits
+    buffer = torch.randn(6, 40, device=dev)
+    left, right = buffer[:, :16], buffer[:, 16:32]
+    want = process_logits(left.clone(), temperature=2.0)
+    assert torch.equal(process_logits(left, temperature=2.0, out=right), want)       # rows in turn, apart
+    assert torch.equal(process_logits(left, temperature=2.0, out=left), want)        # in place
+    keep = buffer.clone()
+    flat = buffer.view(-1)
+    for x, out in ((buffer[:, :16], buffer[:, 15:31]), (buffer[:5, :16], buffer[1:, :16]), (flat[:160].view(10, 16), flat[1:161].view(10, 16)),
+                   (flat[:16].expand(10, 16), flat[:160].view(10, 16))):
+        with pytest.raises(ValueError, match="overlaps the logits"):
+            process_logits(x, out=out)
+    x = torch.randn(6, 16, device=dev)
+    for name, kind in (("bias", dict(bias=left[0])), ("bias", dict(bias=flat[3:19])), ("temperature", dict(temperature=left[2, 3:4])),
+                       ("mask", dict(mask=left[1, :1].view(torch.int32))), ("history", dict(history=right[2, :4].view(torch.int32)))):
+        out = right if name == "history" else left
+        with pytest.raises(ValueError, match=f"out overlaps {name}"):
+            process_logits(x, out=out, **kind)
+    assert torch.equal(process_logits(x, bias=buffer[2, 24:40], out=left), process_logits(x, bias=keep[2, 24:40].clone()))   # between out's rows
+    assert torch.equal(buffer[:, 32:], keep[:, 32:])

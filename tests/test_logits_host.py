@@ -198,3 +198,20 @@ def test_tangents_are_refused(name, grad):
         given[name] = fwAD.make_dual(given[name].requires_grad_(grad and name != "out"), torch.ones_like(given[name]))
         with pytest.raises(L.GcnHipError, match=f"{name} carries a tangent"):
             process_logits(given.pop("logits"), **given)
+
+
+def test_rows_that_meet_against_the_elements_they_hold():
+    """Views [rows, n] of one buffer, their rows dense: they meet if they share an element."""
+    meet = L.binding().rows_meet
+    base = torch.zeros(60)
+    views = [base.as_strided((rows, n), (step, 1), at) for rows in (1, 2, 4) for n in (1, 3, 7) for step in (n, n + 1, 9, 12) if step >= n
+             for at in (0, 1, 5, 8, 13) if at + (rows - 1) * step + n <= 60]
+    shared = [base.as_strided((3, 4), (0, 1), at) for at in (0, 6, 30)]           # expanded: read, never written
+    cells = lambda v: {v.storage_offset() + i * v.stride(0) + j for i in range(v.shape[0]) for j in range(v.shape[1])}
+    met = 0
+    for a in views:
+        for b in views + shared:
+            want = bool(cells(a) & cells(b))
+            assert meet(a, b) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+            met += want
+    assert 0 < met < len(views) * len(views)
