@@ -17,6 +17,7 @@
 #include <cmath>
 #include <cstddef>
 #include <cstring>
+#include <memory>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -80,10 +81,11 @@ struct List {
     std::vector<void*> ptr;
     bool given = false;
 
-    List(const char* name, py::handle h) : name(name) {
+    // own: the tensors outlive the caller's list
+    List(const char* name, py::handle h, bool own = false) : name(name) {
         if (h.is_none()) return;
         given = true;
-        held = py::reinterpret_steal<py::object>(PySequence_Fast(h.ptr(), text(name, " is a list of tensors").c_str()));
+        held = py::reinterpret_steal<py::object>(own ? PySequence_Tuple(h.ptr()) : PySequence_Fast(h.ptr(), text(name, " is a list of tensors").c_str()));
         if (!held) throw py::error_already_set();
         const Py_ssize_t n = PySequence_Fast_GET_SIZE(held.ptr());
         PyObject** items = PySequence_Fast_ITEMS(held.ptr());
@@ -143,63 +145,95 @@ std::vector<int64_t> sizes_of(const List& l) {
     return n;
 }
 
-void adamw_step(py::handle params_, py::handle grads_, py::handle exp_avgs_, py::handle exp_avg_sqs_, py::handle masters_, py::handle exps_,
-                py::handle sq_exps_, long long step, double lr, double beta1, double beta2, double eps, double weight_decay,
-                unsigned long long seed, unsigned int first_tensor, py::handle grad_scale, py::handle clip_coef, py::handle hyper_) {
-    List params("params", params_), grads("grads", grads_), m("exp_avgs", exp_avgs_), v("exp_avg_sqs", exp_avg_sqs_), masters("masters", masters_),
-        em("exp_avg_exps", exps_), ev("exp_avg_sq_exps", sq_exps_);
-    if (em.given != ev.given) value_error("exp_avg_exps and exp_avg_sq_exps go together");
-    const at::ScalarType type = one_type(params, "parameters");
-    const bool half = !params.t.empty() && type != at::kFloat, eight = em.given;
-    const std::vector<int64_t> sizes = sizes_of(params);
-    params.check(sizes, type);
-    grads.check(sizes, type);
-    if (!params.t.empty() && half != masters.given) value_error("master copies go with 16-bit parameters, and only with them");
-    m.check(sizes, eight ? at::kByte : at::kFloat);
-    v.check(sizes, eight ? at::kByte : at::kFloat);
-    if (half) masters.check(sizes, at::kFloat);
-    if (eight) {
-        em.check(sizes, at::kByte, GCN_STATE8_BLOCK);
-        ev.check(sizes, at::kByte, GCN_STATE8_BLOCK);
+// An AdamW step on lists of tensors in two parts: all that can be refused, and the launch.
+struct AdamwCall {
+    List params, grads, m, v, masters, em, ev;
+    at::ScalarType type;
+    bool eight;
+    std::vector<int64_t> sizes;
+    c10::Device d = at::kCPU;
+
+    AdamwCall(py::handle params_, py::handle grads_, py::handle exp_avgs_, py::handle exp_avg_sqs_, py::handle masters_, py::handle exps_,
+              py::handle sq_exps_, bool own)
+        : params("params", params_, own), grads("grads", grads_, own), m("exp_avgs", exp_avgs_, own), v("exp_avg_sqs", exp_avg_sqs_, own),
+          masters("masters", masters_, own), em("exp_avg_exps", exps_, own), ev("exp_avg_sq_exps", sq_exps_, own) {
+        if (em.given != ev.given) value_error("exp_avg_exps and exp_avg_sq_exps go together");
+        type = one_type(params, "parameters");
+        const bool half = !params.t.empty() && type != at::kFloat;
+        eight = em.given;
+        sizes = sizes_of(params);
+        params.check(sizes, type);
+        grads.check(sizes, type);
+        if (!params.t.empty() && half != masters.given) value_error("master copies go with 16-bit parameters, and only with them");
+        m.check(sizes, eight ? at::kByte : at::kFloat);
+        v.check(sizes, eight ? at::kByte : at::kFloat);
+        if (half) masters.check(sizes, at::kFloat);
+        if (eight) {
+            em.check(sizes, at::kByte, GCN_STATE8_BLOCK);
+            ev.check(sizes, at::kByte, GCN_STATE8_BLOCK);
+        }
+        if (params.t.empty()) return;
+        d = params.t[0]->device();
+        need_gpu(*params.t[0], "tensor");
+        for (List* l : {&params, &grads, &m, &v, &masters, &em, &ev}) l->place(d, l != &grads);
+        // a tensor twice, or a part of another, would be updated by two workgroups at once
+        const size_t width = half ? 2 : 4;
+        std::vector<std::pair<const char*, const char*>> once;
+        for (size_t k = 0; k < sizes.size(); ++k)
+            if (sizes[k] > 0) once.emplace_back(static_cast<char*>(params.ptr[k]), static_cast<char*>(params.ptr[k]) + sizes[k] * width);
+        std::sort(once.begin(), once.end());
+        for (size_t k = 1; k < once.size(); ++k) {
+            if (once[k].first == once[k - 1].first) value_error("a parameter is in the list twice");
+            if (once[k].first < once[k - 1].second) value_error("parameters overlap in memory");
+        }
     }
-    if (params.t.empty()) return;
-    const c10::Device d = params.t[0]->device();
-    need_gpu(*params.t[0], "tensor");
-    for (List* l : {&params, &grads, &m, &v, &masters, &em, &ev}) l->place(d, l != &grads);
-    // a tensor twice, or a part of another, would be updated by two workgroups at once
-    const size_t width = half ? 2 : 4;
-    std::vector<std::pair<const char*, const char*>> once;
-    for (size_t k = 0; k < sizes.size(); ++k)
-        if (sizes[k] > 0) once.emplace_back(static_cast<char*>(params.ptr[k]), static_cast<char*>(params.ptr[k]) + sizes[k] * width);
-    std::sort(once.begin(), once.end());
-    for (size_t k = 1; k < once.size(); ++k) {
-        if (once[k].first == once[k - 1].first) value_error("a parameter is in the list twice");
-        if (once[k].first < once[k - 1].second) value_error("parameters overlap in memory");
+    gcn_adamw_desc describe(double lr, double beta1, double beta2, double eps, double weight_decay) const {
+        gcn_adamw_desc desc = {};
+        desc.param_type = type_id(type);
+        desc.state_bits = eight ? 8 : 32;
+        desc.lr = lr; desc.beta1 = beta1; desc.beta2 = beta2; desc.eps = eps; desc.weight_decay = weight_decay;
+        return desc;
     }
-    const void* hyper = nullptr;
-    if (!hyper_.is_none()) {
-        const at::Tensor* t = as_tensor(hyper_);
-        if (!t || t->scalar_type() != at::kByte || t->device() != d || static_cast<size_t>(t->numel()) < api.adamw_hyper_bytes())
-            value_error("hyper is what adamw_hyper returned, on the tensors' device");
-        hyper = t->const_data_ptr();
+    // what run() would refuse of these
+    void check_numbers(double lr, double beta1, double beta2, double eps, double weight_decay, py::handle grad_scale) const {
+        if (params.t.empty()) return;
+        device_scalar(grad_scale, "grad_scale", d);
+        gcn_adamw_desc desc = describe(lr, beta1, beta2, eps, weight_decay);
+        desc.step = 1;                              // and no tensors: nothing is launched
+        check(api.adamw_step(&desc, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr), "gcn_adamw_step");
     }
-    const float *scale = device_scalar(grad_scale, "grad_scale", d), *clip = device_scalar(clip_coef, "clip_coef", d);
-    c10::DeviceGuard guard(d);
-    if (!hyper && capturing()) gcn_error("a captured step would repeat its step count: pass hyper (adamw_advance_)");
-    gcn_adamw_desc desc = {};
-    desc.n = static_cast<int>(sizes.size());
-    desc.param_type = type_id(type);
-    desc.state_bits = eight ? 8 : 32;
-    desc.first_tensor = first_tensor;
-    desc.lr = lr; desc.beta1 = beta1; desc.beta2 = beta2; desc.eps = eps; desc.weight_decay = weight_decay;
-    desc.step = step;
-    desc.seed = seed;
-    static_assert(sizeof(long long) == sizeof(int64_t), "sizes are handed over as they are");
-    check(api.adamw_step(&desc, params.table(), grads.table(), reinterpret_cast<float* const*>(masters.table()), m.table(), v.table(),
-                         reinterpret_cast<unsigned char* const*>(em.table()), reinterpret_cast<unsigned char* const*>(ev.table()),
-                         reinterpret_cast<const long long*>(sizes.data()), scale, clip, hyper, stream_of(d)),
-          "gcn_adamw_step");
-    for (const List* l : {&params, &m, &v, &masters, &em, &ev}) l->written();
+    void run(long long step, double lr, double beta1, double beta2, double eps, double weight_decay, unsigned long long seed,
+             unsigned int first_tensor, py::handle grad_scale, py::handle clip_coef, py::handle hyper_) const {
+        if (params.t.empty()) return;
+        const void* hyper = nullptr;
+        if (!hyper_.is_none()) {
+            const at::Tensor* t = as_tensor(hyper_);
+            if (!t || t->scalar_type() != at::kByte || t->device() != d || static_cast<size_t>(t->numel()) < api.adamw_hyper_bytes())
+                value_error("hyper is what adamw_hyper returned, on the tensors' device");
+            hyper = t->const_data_ptr();
+        }
+        const float *scale = device_scalar(grad_scale, "grad_scale", d), *clip = device_scalar(clip_coef, "clip_coef", d);
+        c10::DeviceGuard guard(d);
+        if (!hyper && capturing()) gcn_error("a captured step would repeat its step count: pass hyper (adamw_advance_)");
+        gcn_adamw_desc desc = describe(lr, beta1, beta2, eps, weight_decay);
+        desc.n = static_cast<int>(sizes.size());
+        desc.first_tensor = first_tensor;
+        desc.step = step;
+        desc.seed = seed;
+        static_assert(sizeof(long long) == sizeof(int64_t), "sizes are handed over as they are");
+        check(api.adamw_step(&desc, params.table(), grads.table(), reinterpret_cast<float* const*>(masters.table()), m.table(), v.table(),
+                             reinterpret_cast<unsigned char* const*>(em.table()), reinterpret_cast<unsigned char* const*>(ev.table()),
+                             reinterpret_cast<const long long*>(sizes.data()), scale, clip, hyper, stream_of(d)),
+              "gcn_adamw_step");
+        for (const List* l : {&params, &m, &v, &masters, &em, &ev}) l->written();
+    }
+};
+
+void adamw_step(py::handle params, py::handle grads, py::handle exp_avgs, py::handle exp_avg_sqs, py::handle masters, py::handle exps, py::handle sq_exps,
+                long long step, double lr, double beta1, double beta2, double eps, double weight_decay, unsigned long long seed,
+                unsigned int first_tensor, py::handle grad_scale, py::handle clip_coef, py::handle hyper) {
+    AdamwCall(params, grads, exp_avgs, exp_avg_sqs, masters, exps, sq_exps, false)
+        .run(step, lr, beta1, beta2, eps, weight_decay, seed, first_tensor, grad_scale, clip_coef, hyper);
 }
 
 py::tuple grad_norm(py::handle grads_, py::handle max_norm_, py::handle grad_scale) {
@@ -578,6 +612,11 @@ void bind(const py::dict& addresses, py::object error) {
 PYBIND11_MODULE(gcn_uelb_torch, m) {
     m.def("bind", &bind);
     m.def("adamw_step", &adamw_step);
+    py::class_<AdamwCall>(m, "AdamwCall")
+        .def(py::init([](py::handle params, py::handle grads, py::handle exp_avgs, py::handle exp_avg_sqs, py::handle masters, py::handle exps,
+                         py::handle sq_exps) { return std::make_unique<AdamwCall>(params, grads, exp_avgs, exp_avg_sqs, masters, exps, sq_exps, true); }))
+        .def("check_numbers", &AdamwCall::check_numbers)
+        .def("run", &AdamwCall::run);
     m.def("grad_norm", &grad_norm);
     m.def("process_logits", &process_logits);
     m.def("row_stride", [](const at::Tensor& t, int64_t dim) { return row_stride(t, dim); });

@@ -46,6 +46,11 @@ def adamw_hyper(device):
     return torch.zeros(L.load().gcn_adamw_hyper_bytes(), dtype=torch.uint8, device=device)
 
 
+def _check_device_lr(lr, device):
+    if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
+        raise TypeError("lr on the device is a float32 tensor of one element, where step is")
+
+
 def adamw_advance_(step, hyper, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0):
     """Adds 1 to ``step`` (an int64 scalar on the device) and puts what ``adamw_step_`` needs for that step into ``hyper``, both on
     the device, so that a captured graph counts on when it is replayed.  lr: a number, or a float32 scalar on the device."""
@@ -57,10 +62,10 @@ def adamw_advance_(step, hyper, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_deca
     if hyper.device != dev or hyper.dtype != torch.uint8 or hyper.numel() < lib.gcn_adamw_hyper_bytes():
         raise ValueError("hyper is what adamw_hyper returned, on step's device")
     on_device = isinstance(lr, torch.Tensor)
+    if on_device:
+        _check_device_lr(lr, dev)
     desc = L.AdamWDesc(n=0, state_bits=32, lr=0.0 if on_device else lr, beta1=betas[0], beta2=betas[1], eps=eps,
                        weight_decay=weight_decay, seed=seed)
-    if on_device and (lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev):
-        raise TypeError("lr on the device is a float32 tensor of one element, where step is")
     with L.device_guard(dev):
         rc = lib.gcn_adamw_advance(ctypes.byref(desc), step.data_ptr(), lr.data_ptr() if on_device else None, hyper.data_ptr(), L.stream_ptr(dev))
     L.check(rc, "gcn_adamw_advance")
@@ -127,6 +132,8 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f"Invalid state_bits (8 or 32): {state_bits}")
         if max_grad_norm is not None and not max_grad_norm >= 0:
             raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
+        if not 0 <= seed < 1 << 64:
+            raise ValueError(f"Invalid seed: {seed}")
         self.state_bits, self.min_8bit_numel, self.max_grad_norm = state_bits, min_8bit_numel, max_grad_norm
         self.capturable, self.seed = capturable, seed
         self.grad_norm = None
@@ -171,16 +178,18 @@ class FusedAdamW(torch.optim.Optimizer):
             raise RuntimeError("FusedAdamW needs contiguous parameters")
 
     def _collect(self):
-        """[(group, step tensor, number of the group's first parameter, parameters, gradients, states)]: what is updated together:
-        one type, one device, one width of states, one step count.  New parameters get their states here."""
-        jobs, first = [], 0
+        """(jobs, made, idle).  jobs: [(group, step tensor, number of the group's first parameter, parameters, gradients, states)]:
+        what is updated together: one type, one device, one width of states, one step count.  made: [(parameter, state)] for new
+        parameters, idle: states without a gradient that share a step tensor with updated ones; ``step`` adopts both once
+        nothing can be refused any more."""
+        jobs, made, idle, first = [], [], [], 0
         for group in self.param_groups:
-            buckets, idle, fresh = {}, [], {}
+            buckets, waiting, fresh = {}, [], {}
             for p in group["params"]:
                 g, st = p.grad, self.state.get(p)
                 if g is None:
                     if st:
-                        idle.append(st)
+                        waiting.append(st)
                     continue
                 if not st:
                     self._check(p)
@@ -189,9 +198,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     step = fresh.setdefault(p.device, None)
                     if step is None:
                         step = fresh[p.device] = self._new_step(p.device)
-                    st = self.state[p]
-                    st["step"] = step
-                    st.update(self._zero_state(p))
+                    st = {"step": step, **self._zero_state(p)}
+                    made.append((p, st))
                 step = st["step"]
                 bucket = buckets.get((id(step), p.dtype, p.device, "exp_avg_exp" in st))
                 if bucket is None:
@@ -201,14 +209,25 @@ class FusedAdamW(torch.optim.Optimizer):
                 bucket[5].append(st)
             # parameters without a gradient keep their count: a step tensor that they share with updated ones is copied for them
             counted = {id(b[1]) for b in buckets.values()}
-            for st in idle:
-                if id(st["step"]) in counted:
-                    if torch.cuda.is_current_stream_capturing():
-                        raise L.GcnHipError("FusedAdamW: a parameter had a gradient before capture and has none now")
-                    st["step"] = st["step"].clone()
+            idle += [st for st in waiting if id(st["step"]) in counted]
+            if idle and torch.cuda.is_current_stream_capturing():
+                raise L.GcnHipError("FusedAdamW: a parameter had a gradient before capture and has none now")
             jobs += buckets.values()
             first += len(group["params"])
-        return jobs
+        return jobs, made, idle
+
+    def _prepare(self, group, step, first, params, grads, states, grad_scale):
+        """The checked call of a job: what could be refused has been."""
+        masters, eight = "master" in states[0], "exp_avg_exp" in states[0]
+        call = L.binding().AdamwCall(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                                     [s["master"] for s in states] if masters else None, [s["exp_avg_exp"] for s in states] if eight else None,
+                                     [s["exp_avg_sq_exp"] for s in states] if eight else None)
+        lr = group["lr"]
+        if self.capturable and isinstance(lr, torch.Tensor):
+            _check_device_lr(lr, step.device)
+            lr = 0.0
+        call.check_numbers(lr, *group["betas"], group["eps"], group["weight_decay"], grad_scale)
+        return call
 
     def _clip(self, jobs, max_norm, grad_scale):
         """The clip coefficient over all jobs; also sets ``grad_norm``."""
@@ -226,21 +245,28 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale=None, max_grad_norm=None):
-        """One update.  grad_scale: float32 scalar on the device that the gradients are multiplied by (1 / loss scale).
+        """One update, of all parameters or, where it is refused, of none: nothing is counted then.  grad_scale: float32 scalar on the device that the gradients are multiplied by (1 / loss scale).
         max_grad_norm: in place of the constructor's for this step."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
         L.load()
-        jobs = self._collect()
-        # before anything is counted
+        jobs, made, idle = self._collect()
         if jobs and not self.capturable and torch.cuda.is_current_stream_capturing():
             raise L.GcnHipError("FusedAdamW: a captured step would repeat its step count: pass capturable=True")
+        # all of it is checked before anything is counted or updated: a step that is refused leaves everything as it was
+        calls = [self._prepare(*job, grad_scale) for job in jobs]
         max_norm = self.max_grad_norm if max_grad_norm is None else max_grad_norm
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError(f"Invalid max_grad_norm: {max_norm}")
         coef = self._clip(jobs, max_norm, grad_scale) if max_norm is not None and jobs else None
+        for p, st in made:
+            self.state[p] = st
+        for st in idle:
+            st["step"] = st["step"].clone()
         advanced = {}
-        for group, step, first, params, grads, states in jobs:
+        for (group, step, first, *_), call in zip(jobs, calls):
             options = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], seed=self.seed)
             if id(step) not in advanced:
                 if self.capturable:
@@ -253,15 +279,9 @@ class FusedAdamW(torch.optim.Optimizer):
                     step += 1
                     advanced[id(step)] = int(step.item())
             now = advanced[id(step)]
-            eight = "exp_avg_exp" in states[0]
-            if self.capturable:
-                options["lr"] = 0.0                     # read from hyper
-            adamw_step_(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
-                        step=0 if self.capturable else now, hyper=now if self.capturable else None,
-                        masters=[s["master"] for s in states] if "master" in states[0] else None,
-                        exp_avg_exps=[s["exp_avg_exp"] for s in states] if eight else None,
-                        exp_avg_sq_exps=[s["exp_avg_sq_exp"] for s in states] if eight else None,
-                        grad_scale=grad_scale, clip_coef=coef, first_tensor=first, **options)
+            # capturable: step, lr and what depends on them are read from hyper
+            call.run(0 if self.capturable else now, 0.0 if self.capturable else group["lr"], *group["betas"], group["eps"], group["weight_decay"],
+                     self.seed, first, grad_scale, coef, now if self.capturable else None)
         return loss
 
     # ------------------------------------------------------------------ checkpoints

@@ -138,3 +138,9 @@ def test_oracle_hash_and_rounding_are_unbiased():
     value, exps, _, step = O.encode(x, (r & 0xFFFF).astype(np.int64), False)
     assert set(np.unique(value)) == {1.0, 1.125} and (exps == 120).all()
     assert abs(value.mean() - 1.03) < 5 * step[0] * 0.5 / 256
+
+
+@pytest.mark.parametrize("seed", [-1, 1 << 64])
+def test_seeds_have_64_bits(seed):
+    with pytest.raises(ValueError, match="seed"):
+        A.FusedAdamW([torch.nn.Parameter(torch.ones(3))], seed=seed)

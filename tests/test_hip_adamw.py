@@ -611,3 +611,74 @@ def test_a_refused_capture_counts_no_step(dev, A):
     assert float(opt.state[p]["step"]) == 1 and torch.equal(p.detach(), before)
     opt.step()
     assert float(opt.state[p]["step"]) == 2
+
+
+def _turn(p):
+    p.data = torch.ones(p.shape[::-1], device=p.device).t()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("name", ["layout", "learning rate", "beta", "weight decay", "gradient scale", "norm", "new parameter"])
+def test_a_refused_step_counts_nothing_and_updates_nothing(dev, A, name, capturable):
+    """Two groups, the second of which is refused; afterwards the optimizer goes on as one that was never refused."""
+    def build():
+        a, b = model(dev)[:2], model(dev, torch.bfloat16, seed=3)[:2]
+        opt = A.FusedAdamW([{"params": a}, {"params": b}], lr=1e-2, capturable=capturable, max_grad_norm=1.0)
+        feed_grads(a + b, 0)
+        opt.step()
+        return a, b, opt
+
+    a, b, opt = build()
+    before = [[x.clone() for x in (p.detach(), *(v for k, v in sorted(opt.state[p].items())))] for p in a + b]
+    group, kind, new = opt.param_groups[1], {}, []
+    if name == "layout":
+        keep = b[0].data
+        _turn(b[0])
+    elif name == "learning rate":
+        group["lr"] = torch.tensor(1e-2, dtype=torch.float64, device=dev) if capturable else -1.0
+    elif name == "beta":
+        group["betas"] = (0.9, 1.0)
+    elif name == "weight decay":
+        group["weight_decay"] = -0.5
+    elif name == "gradient scale":
+        kind["grad_scale"] = torch.ones((), dtype=torch.float64, device=dev)
+    elif name == "norm":
+        kind["max_grad_norm"] = -1.0
+    else:
+        new = [torch.nn.Parameter(torch.ones(5, device=dev)), torch.nn.Parameter(torch.ones(8, 4, device=dev).t())]
+        opt.add_param_group({"params": new})
+        for q in new:
+            q.grad = torch.ones_like(q)
+    feed_grads(a + b, 1)
+    with pytest.raises((ValueError, TypeError, RuntimeError)):
+        opt.step(**kind)
+    if name == "layout":
+        b[0].data = keep
+    for p, want in zip(a + b, before):
+        now = [p.detach(), *(v for k, v in sorted(opt.state[p].items()))]
+        assert len(now) == len(want) and all(torch.equal(x, y) for x, y in zip(now, want))
+    assert not any(opt.state.get(q) for q in new)
+    # mended, it goes on
+    group.update(lr=1e-2, betas=(0.9, 0.999), weight_decay=1e-2)
+    for q in new:
+        q.grad = None
+    other_a, other_b, other = build()
+    for ps, o in ((a + b, opt), (other_a + other_b, other)):
+        feed_grads(ps, 1)
+        o.step()
+    assert all(torch.equal(x, y) for x, y in zip(a + b, other_a + other_b))
+    assert {int(opt.state[p]["step"]) for p in a + b} == {2}
+
+
+def test_a_call_keeps_its_tensors(dev, A):
+    """What the optimizer prepares outlives the lists that it was made from."""
+    from src.gcn.hip import lib as L
+    p, g = [torch.ones(1000, device=dev)], [torch.ones(1000, device=dev)]
+    m, v = [torch.zeros(1000, device=dev)], [torch.zeros(1000, device=dev)]
+    keep = p[0]
+    call_ = L.binding().AdamwCall(p, g, m, v, None, None, None)
+    for ts in (p, g, m, v):
+        ts.clear()
+    junk = [torch.full((1000,), 7.0, device=dev) for _ in range(4)]
+    call_.run(1, 0.5, 0.9, 0.999, 1e-8, 0.0, 0, 0, None, None, None)
+    assert float((keep - 0.5).abs().max()) <= 1e-6 and all(bool((j == 7).all()) for j in junk)
