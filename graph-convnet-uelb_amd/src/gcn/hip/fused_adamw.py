@@ -1,7 +1,8 @@
 """Multi-tensor AdamW on the HIP library, with moments in fp32 or in 8 bits, and the global gradient norm it clips by.
 
 ``FusedAdamW`` is used like ``torch.optim.AdamW`` (the reference trains with ``torch.optim.Adam`` only,
-``src/gcn/train/trainer.py:95``): the same constructor arguments and ``param_groups``, and with 32-bit states the same
+``src/gcn/train/trainer.py:95``): the same constructor arguments but for amsgrad, maximize, foreach,
+differentiable and fused, the same ``param_groups``, and with 32-bit states the same
 ``state_dict`` layout, so optimizer checkpoints move between the two.  ``adamw_step_`` and ``grad_norm`` are the same
 operations on lists of tensors.  Formulas, formats and what the kernels do are described in ``include/gcn_uelb_hip.h``.
 
@@ -139,6 +140,19 @@ class FusedAdamW(torch.optim.Optimizer):
         self.grad_norm = None
         self._hyper = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    @staticmethod
+    def _refuse_options(group):
+        """Options of ``torch.optim.AdamW`` that change the update and that this optimizer does not have (foreach, fused and
+        capturable change none)."""
+        for name in ("amsgrad", "maximize", "differentiable"):
+            if group.get(name):
+                raise ValueError(f"FusedAdamW does not support {name}")
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            self._refuse_options(param_group)
+        super().add_param_group(param_group)
 
     # ------------------------------------------------------------------ states
     def _bits(self, p):
@@ -299,24 +313,41 @@ class FusedAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes states of this optimizer or of ``torch.optim.AdamW`` / ``Adam`` over the same parameters; moments are converted to
-        this optimizer's width."""
+        this optimizer's width.  Refused are amsgrad, maximize, differentiable and a weight decay that is part of the gradient;
+        nothing is loaded then."""
+        groups = state_dict["param_groups"]
+        for group in groups:
+            self._refuse_options(group)
+            if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
+                raise ValueError("the saved optimizer adds its weight decay to the gradient, which AdamW does not")
+        # all states before anything is replaced; the base class refuses groups that do not match
+        made, shared = [], {}
+        if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:
+            ids = itertools.chain.from_iterable(g["params"] for g in groups)
+            for sid, (group_no, p) in zip(ids, ((k, p) for k, g in enumerate(self.param_groups) for p in g["params"])):
+                saved = state_dict["state"].get(sid)
+                if not saved:
+                    continue
+                st = self._from_saved(p, saved)
+                key = (group_no, p.device, int(saved["step"]))
+                if key not in shared:
+                    shared[key] = self._new_step(p.device, int(saved["step"]))
+                st["step"] = shared[key]
+                made.append((p, st))
         super().load_state_dict(state_dict)
         # the base class casts every state to its parameter's type: take them as they were saved
-        ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
-        shared = {}
-        for sid, (group_no, p) in zip(ids, ((k, p) for k, g in enumerate(self.param_groups) for p in g["params"])):
-            saved = state_dict["state"].get(sid)
-            if not saved:
-                continue
-            st = self._from_saved(p, saved)
-            key = (group_no, p.device, int(saved["step"]))
-            if key not in shared:
-                shared[key] = self._new_step(p.device, int(saved["step"]))
-            st["step"] = shared[key]
+        for p, st in made:
             self.state[p] = st
+        for group in self.param_groups:
+            if "decoupled_weight_decay" in group:
+                group["decoupled_weight_decay"] = True
         self._hyper = {}
 
     def _from_saved(self, p, saved):
+        if "max_exp_avg_sq" in saved:
+            raise ValueError("FusedAdamW has no amsgrad: the saved state holds the largest second moments")
+        if "step" not in saved:
+            raise ValueError("the saved state holds no step count")
         st = {k: saved[k].to(p.device, copy=True).contiguous() for k in _KEPT if k in saved}
         for key in ("exp_avg", "exp_avg_sq"):
             if key not in st or st[key].numel() != p.numel():

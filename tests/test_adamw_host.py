@@ -144,3 +144,57 @@ def test_oracle_hash_and_rounding_are_unbiased():
 def test_seeds_have_64_bits(seed):
     with pytest.raises(ValueError, match="seed"):
         A.FusedAdamW([torch.nn.Parameter(torch.ones(3))], seed=seed)
+
+
+@pytest.mark.parametrize("source, change", [
+    (torch.optim.AdamW, dict(amsgrad=True)), (torch.optim.AdamW, dict(maximize=True)), (torch.optim.AdamW, dict(differentiable=True)),
+    (torch.optim.Adam, dict(weight_decay=0.1)), (torch.optim.AdamW, "max_exp_avg_sq"), (torch.optim.AdamW, "step"), (torch.optim.AdamW, "size"),
+    (torch.optim.AdamW, "groups")])
+def test_checkpoints_of_another_update_are_refused(source, change):
+    """Each of them changes what a step does; nothing of a refused checkpoint is loaded."""
+    theirs = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(4))]
+    opt = source(theirs, lr=0.5, foreach=False, **(change if isinstance(change, dict) else {}))
+    for p in theirs:
+        p.grad = torch.ones_like(p)
+    if change != dict(differentiable=True):
+        opt.step()
+    saved = opt.state_dict()
+    if change == "max_exp_avg_sq":
+        saved["state"][1]["max_exp_avg_sq"] = torch.ones(4)
+    elif change == "step":
+        del saved["state"][1]["step"]
+    elif change == "size":
+        saved["state"][1]["exp_avg"] = torch.ones(5)
+    elif change == "groups":
+        saved["param_groups"][0]["params"] = [0]
+    ours = A.FusedAdamW([torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(4))], lr=1e-3)
+    with pytest.raises(ValueError):
+        ours.load_state_dict(saved)
+    assert not ours.state and ours.param_groups[0]["lr"] == 1e-3 and "maximize" not in ours.param_groups[0]
+
+
+def test_groups_with_options_of_another_update_are_refused():
+    p = lambda: torch.nn.Parameter(torch.ones(3))
+    for name in ("amsgrad", "maximize", "differentiable"):
+        with pytest.raises(ValueError, match=name):
+            A.FusedAdamW([{"params": [p()], name: True}])
+        opt = A.FusedAdamW([{"params": [p()], name: False}])
+        with pytest.raises(ValueError, match=name):
+            opt.add_param_group({"params": [p()], name: True})
+        assert len(opt.param_groups) == 1
+
+
+@pytest.mark.parametrize("source", [torch.optim.AdamW, torch.optim.Adam])
+def test_checkpoints_of_the_same_update_are_taken(source):
+    theirs = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(4))]
+    opt = source(theirs, lr=0.5, foreach=False)
+    for p in theirs:
+        p.grad = torch.full_like(p, 2.0)
+    opt.step()
+    mine = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(4))]
+    ours = A.FusedAdamW(mine)
+    ours.load_state_dict(opt.state_dict())
+    assert ours.param_groups[0]["lr"] == 0.5 and ours.param_groups[0]["decoupled_weight_decay"] is True
+    for p, q in zip(mine, theirs):
+        assert torch.equal(ours.state[p]["exp_avg"], opt.state[q]["exp_avg"]) and float(ours.state[p]["step"]) == 1
+    assert ours.state[mine[0]]["step"] is ours.state[mine[1]]["step"]
