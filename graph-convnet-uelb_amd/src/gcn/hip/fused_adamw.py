@@ -192,8 +192,8 @@ class FusedAdamW(torch.optim.Optimizer):
             raise RuntimeError("FusedAdamW needs contiguous parameters")
 
     def _collect(self):
-        """(jobs, made, idle).  jobs: [(group, step tensor, number of the group's first parameter, parameters, gradients, states)]:
-        what is updated together: one type, one device, one width of states, one step count.  made: [(parameter, state)] for new
+        """(jobs, made, idle).  jobs: [[group, step tensor, number of the first tensor, parameters, gradients, states]]: what is
+        updated together: one type, one device, one width of states, one step count.  made: [(parameter, state)] for new
         parameters, idle: states without a gradient that share a step tensor with updated ones; ``step`` adopts both once
         nothing can be refused any more."""
         jobs, made, idle, first = [], [], [], 0
@@ -217,7 +217,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 step = st["step"]
                 bucket = buckets.get((id(step), p.dtype, p.device, "exp_avg_exp" in st))
                 if bucket is None:
-                    bucket = buckets[(id(step), p.dtype, p.device, "exp_avg_exp" in st)] = (group, step, first, [], [], [])
+                    bucket = buckets[(id(step), p.dtype, p.device, "exp_avg_exp" in st)] = [group, step, first, [], [], []]
                 bucket[3].append(p)
                 bucket[4].append(g if g.is_contiguous() else g.contiguous())
                 bucket[5].append(st)
@@ -226,6 +226,13 @@ class FusedAdamW(torch.optim.Optimizer):
             idle += [st for st in waiting if id(st["step"]) in counted]
             if idle and torch.cuda.is_current_stream_capturing():
                 raise L.GcnHipError("FusedAdamW: a parameter had a gradient before capture and has none now")
+            # 8-bit tensors are numbered one after the other, also where a group falls into several lists: the numbers enter the
+            # random bits of the rounding
+            number = first
+            for job in buckets.values():
+                if "exp_avg_exp" in job[5][0]:
+                    job[2] = number
+                    number += len(job[3])
             jobs += buckets.values()
             first += len(group["params"])
         return jobs, made, idle

@@ -682,3 +682,43 @@ def test_a_call_keeps_its_tensors(dev, A):
     junk = [torch.full((1000,), 7.0, device=dev) for _ in range(4)]
     call_.run(1, 0.5, 0.9, 0.999, 1e-8, 0.0, 0, 0, None, None, None)
     assert float((keep - 0.5).abs().max()) <= 1e-6 and all(bool((j == 7).all()) for j in junk)
+
+
+@pytest.mark.parametrize("why", ["types", "step counts"])
+def test_lists_of_one_group_round_with_bits_of_their_own(dev, A, why):
+    """A group that falls into several 8-bit lists: equal values and gradients in each, and the oracle's bits for the tensors numbered one
+    after the other.  Equal bits would give equal codes; of 4096 elements rounded at random about half or more differ."""
+    n = 4096
+    grads = [torch.from_numpy(np.random.default_rng(7).standard_normal(n).astype(np.float32)).to(torch.bfloat16).float().to(dev) for _ in range(4)]
+    types = [torch.float32, torch.bfloat16, torch.float32, torch.bfloat16] if why == "types" else [torch.float32] * 4
+    small = torch.nn.Parameter(torch.ones(8, device=dev))                    # fp32 moments: takes no number
+    params = [torch.nn.Parameter(torch.ones(n, device=dev, dtype=t)) for t in types]
+    opt = A.FusedAdamW([small, *params], lr=1e-2, state_bits=8, seed=5)
+    small.grad = torch.ones_like(small)
+    if why == "step counts":                                                  # two of them miss a step; then all states are made equal
+        for p in params[:2]:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        for p in params[2:]:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        for p in params:
+            for key in ("exp_avg", "exp_avg_sq", "exp_avg_exp", "exp_avg_sq_exp"):
+                opt.state[p][key].zero_()
+        with torch.no_grad():
+            for p in params[2:]:
+                opt.state[p]["step"].fill_(2.0)                               # a count of their own, of the same value
+    for p, g in zip(params, grads):
+        p.grad = g.to(p.dtype)
+    opt.step()
+    codes = [opt.state[p]["exp_avg"].cpu().numpy() for p in params]
+    for i in range(4):
+        for j in range(i):
+            assert (codes[i] != codes[j]).mean() > 0.25, (i, j)
+    step = 1 if why == "types" else 3
+    order = [0, 2, 1, 3] if why == "types" else [0, 1, 2, 3]
+    m = (np.float32(1 - 0.9) * grads[0].cpu().numpy()).astype(np.float64)
+    for number, k in enumerate(order):
+        want, exps, margin, unit = O.encode(m, (O.random32(n, 5, step, number) & 0xFFFF).astype(np.int64), False)
+        off = np.abs(O.decode(codes[k], opt.state[params[k]]["exp_avg_exp"].cpu().numpy()) - want)
+        assert ((off == 0) | (margin * unit <= 4 * U * np.abs(m))).all()
