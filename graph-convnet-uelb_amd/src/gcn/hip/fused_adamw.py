@@ -284,8 +284,12 @@ class FusedAdamW(torch.optim.Optimizer):
         coef = self._clip(jobs, max_norm, grad_scale) if max_norm is not None and jobs else None
         for p, st in made:
             self.state[p] = st
+        copies = {}                 # those that shared a count go on sharing one, and will be one list again
         for st in idle:
-            st["step"] = st["step"].clone()
+            step = st["step"]
+            if id(step) not in copies:
+                copies[id(step)] = (step, step.clone())
+            st["step"] = copies[id(step)][1]
         advanced = {}
         for (group, step, first, *_), call in zip(jobs, calls):
             options = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], seed=self.seed)

@@ -722,3 +722,19 @@ def test_lists_of_one_group_round_with_bits_of_their_own(dev, A, why):
         want, exps, margin, unit = O.encode(m, (O.random32(n, 5, step, number) & 0xFFFF).astype(np.int64), False)
         off = np.abs(O.decode(codes[k], opt.state[params[k]]["exp_avg_exp"].cpu().numpy()) - want)
         assert ((off == 0) | (margin * unit <= 4 * U * np.abs(m))).all()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_parameters_that_skip_a_step_together_stay_one_list(dev, A, capturable):
+    """Ten parameters without a gradient for a step, three of them for another: lists afterwards, and counts."""
+    params = [torch.nn.Parameter(torch.ones(20 + k, device=dev)) for k in range(16)]
+    opt = A.FusedAdamW(params, lr=1e-2, capturable=capturable)
+    lists = []
+    for skipped in ((), range(6, 16), (), range(13, 16), ()):
+        for k, p in enumerate(params):
+            p.grad = None if k in skipped else torch.ones_like(p)
+        lists.append(len(opt._collect()[0]))
+        opt.step()
+    assert lists == [1, 1, 2, 2, 3]
+    assert [int(opt.state[p]["step"]) for p in params] == [5] * 6 + [4] * 7 + [3] * 3
+    assert len({id(opt.state[p]["step"]) for p in params}) == 3
