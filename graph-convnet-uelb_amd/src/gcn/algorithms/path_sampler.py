@@ -178,6 +178,12 @@ class PathSampler:
                                                      float(self.top_p), float(self.entropy_epsilon), _rng_words(self.device), None)
         return paths, plen
 
+    def draw_with_log_probs(self):
+        """``draw`` with the paths' log-probabilities [B], attached to the scores as those of ``sample`` are."""
+        logp_b, paths, plen, *_ = PathLogProbFn.apply(self.y_pred_edges.float().contiguous(), self._cap, self._comm, float(self.temperature),
+                                                      float(self.top_p), float(self.entropy_epsilon), _rng_words(self.device), None)
+        return paths, plen, logp_b
+
     def sample(self):
         """Returns (batch_paths[b][c], log_probs_tensor [B], is_feasible, batch_stepwise_entropies[b][c][step])."""
         return self._finish(*self._run())

@@ -99,7 +99,8 @@ class ReinforcementLearningStrategy(BaseTrainingStrategy):
         self.grad_clip_max_norm = g('rl_grad_clip_max_norm', 1.0)
         self.last_grad_explosion = False
         # penalties for links that a first draw of all commodities uses, applied to the scores before the paths that count are
-        # drawn (LinkScoreRules); neutral by default: one draw on the scores as they are
+        # drawn (LinkScoreRules); neutral by default: one draw on the scores as they are.  The first draw depends on the scores
+        # too: the policy's probability is p(first | scores) p(paths | first, scores), and both enter the gradient
         self.link_penalties = dict(repetition_penalty=g('rl_link_repetition_penalty', 1.0), presence_penalty=g('rl_link_presence_penalty', 0.0),
                                    frequency_penalty=g('rl_link_frequency_penalty', 0.0))
         # test hook: (paths int32 [B,C,PL], path_len int32 [B,C]) to evaluate instead of sampling
@@ -131,14 +132,14 @@ class ReinforcementLearningStrategy(BaseTrainingStrategy):
         dev = y_preds.device
         B = y_preds.shape[0]            # the graphs of this rank's shard (self.batch_size is the global batch)
         sampling = bool(self.use_sampling and model.training)
-        path_log_probs = stepwise = None
+        path_log_probs = stepwise = first_log_probs = None
         if sampling:
             if y_preds.dim() != 4:
                 raise ValueError("path sampling needs edge scores [B,V,V,C] (voc_edges_out == 1)")
             if list(self.link_penalties.values()) != [1.0, 0.0, 0.0]:
-                first = PathSampler(y_pred_edges=y_preds, edges_capacity=cap, commodities=comm, num_samples=1,
-                                    temperature=self.get_current_temperature(), top_p=self.sampling_top_p,
-                                    entropy_epsilon=self.entropy_epsilon).draw()
+                *first, first_log_probs = PathSampler(y_pred_edges=y_preds, edges_capacity=cap, commodities=comm, num_samples=1,
+                                                      temperature=self.get_current_temperature(), top_p=self.sampling_top_p,
+                                                      entropy_epsilon=self.entropy_epsilon).draw_with_log_probs()
                 y_preds = LinkScoreRules(cap, **self.link_penalties)(y_preds, *first)
             sampler = PathSampler(y_pred_edges=y_preds, edges_capacity=cap, commodities=comm, num_samples=1,
                                   temperature=self.get_current_temperature(), top_p=self.sampling_top_p,
@@ -147,6 +148,8 @@ class ReinforcementLearningStrategy(BaseTrainingStrategy):
                 pred_paths, path_log_probs, is_feasible, stepwise = sampler.evaluate(*self.replay_paths)
             else:
                 pred_paths, path_log_probs, is_feasible, stepwise = sampler.sample()
+            if first_log_probs is not None:
+                path_log_probs = path_log_probs + first_log_probs
             max_lf, complete, plen = sampler.max_load_factor, sampler.complete, sampler.path_len
         else:
             bs = BeamSearchFactory.create_algorithm(self.beam_search_type, y_pred_edges=y_preds, beam_size=self.beam_size,

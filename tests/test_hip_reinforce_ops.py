@@ -210,3 +210,107 @@ def test_trainer_epochs_and_checkpoint(dev, tmp_path, monkeypatch, optimizer, st
     assert torch.equal(tr.optimizer.state[p]["exp_avg"], again.optimizer.state[q]["exp_avg"])
     assert float(again.optimizer.state[q]["step"]) == 6
     assert any("exp_avg_exp" in st for st in again.optimizer.state.values()) == (optimizer == "adamw8bit")
+
+
+class FixedScores(torch.nn.Module):
+    def __init__(self, y):
+        super().__init__()
+        self.y = torch.nn.Parameter(y)
+
+    def forward(self, x_edges, x_commodities, cap, x_nodes, y_edges=None, edge_cw=None, compute_loss=False, mask_invalid_edges=False):
+        return self.y, None
+
+
+def test_the_gradient_with_link_penalties_is_that_of_the_expected_reward(dev, monkeypatch):
+    """Two routes, 0 - 1 - 3 and 0 - 2 - 3: the strategy's gradients of all four pairs (first draw, paths that count), weighted with the
+    pairs' probabilities, add up to the derivative of the expected reward over both draws, taken by differences in double
+    precision.  Without the first draw's probability the sum is another one (shown at the end)."""
+    from src.gcn.algorithms.path_sampler import PathLogProbFn, PathSampler
+    from src.gcn.training.reinforcement_strategy import ReinforcementLearningStrategy
+    rho, presence, frequency = 1.4, 0.6, 0.3
+    cfg = dict(rl_use_baseline=False, rl_normalize_advantages=False, rl_entropy_weight=0.0, rl_sampling_temperature=1.0, rl_sampling_top_p=1.0,
+               rl_entropy_epsilon=0.0, rl_link_repetition_penalty=rho, rl_link_presence_penalty=presence, rl_link_frequency_penalty=frequency)
+    cap = torch.zeros(1, 4, 4, device=dev)
+    for i, j, c in ((0, 1, 10.0), (1, 3, 10.0), (0, 2, 3.0), (2, 3, 3.0)):
+        cap[0, i, j] = c
+    comm = torch.tensor([[[0, 3, 2]]], device=dev)
+    path = {k: torch.tensor([[[0, k, 3] + [-1] * 7]], dtype=torch.int32, device=dev) for k in (1, 2)}
+    length = torch.full((1, 1), 3, dtype=torch.int32, device=dev)
+    y = torch.randn(1, 4, 4, 1, generator=torch.Generator().manual_seed(4))
+    y[0, 0, 1, 0], y[0, 0, 2, 0] = 0.7, -0.4                                   # one of either sign
+    data = dict(x_edges=None, x_commodities=comm[:, :, 2].float(), x_edges_capacity=cap, x_nodes=None, batch_commodities=comm)
+    chosen = {}
+
+    def forced(self):
+        logp, paths, plen, *_ = PathLogProbFn.apply(self.y_pred_edges.float().contiguous(), self._cap, self._comm, float(self.temperature),
+                                                    float(self.top_p), float(self.entropy_epsilon), None, (path[chosen["first"]], length))
+        return paths, plen, logp
+    monkeypatch.setattr(PathSampler, "draw_with_log_probs", forced)
+
+    def probabilities(a):
+        """p(first), p(second | first) in double precision from the scores of links 0 - 1 and 0 - 2."""
+        def soft(z):
+            e = np.exp(z - z.max())
+            return e / e.sum()
+        p, q = soft(a), np.empty((2, 2))
+        for f in range(2):
+            z = a.copy()
+            z[f] = (z[f] / rho if z[f] > 0 else z[f] * rho) - presence - frequency
+            q[f] = soft(z)
+        return p, q
+
+    at = np.array([float(y[0, 0, 1, 0]), float(y[0, 0, 2, 0])])
+    p, q = probabilities(at)
+    reward, total, size = {}, np.zeros(2), 0.0
+    for f in (1, 2):
+        for s in (1, 2):
+            chosen["first"] = f
+            strat = ReinforcementLearningStrategy(cfg)
+            strat.replay_paths = (path[s], length)
+            model = FixedScores(y.to(dev)).train()
+            loss, m = strat.compute_loss(model, data, dev)
+            loss.backward()
+            assert not m["reinforce_fallback_used"]
+            reward[s] = m["reward_individual"][0]
+            grad = -model.y.grad.cpu().double().numpy()[0, :, :, 0]
+            weight = p[f - 1] * q[f - 1, s - 1]
+            total += weight * grad[0, 1:3]
+            size += weight * np.abs(grad[0, 1:3]).max()
+            grad[0, 1:3] = 0
+            assert (grad == 0).all()                                            # the other nodes have one way on
+    assert reward[1] != reward[2]
+
+    def expected(a):
+        p, q = probabilities(a)
+        return sum(p[f] * q[f, s] * reward[s + 1] for f in range(2) for s in range(2))
+
+    step, want = 1e-5, np.empty(2)
+    for k in range(2):
+        e = np.eye(2)[k] * step
+        want[k] = (expected(at + e) - expected(at - e)) / (2 * step)
+    # the fp32 softmax, its logarithm and the rules: about 20 roundings of each term; differences: step^2 and 1e-16 / step
+    assert (np.abs(total - want) <= 64 * U * size + 1e-9).all(), (total, want)
+    onehot = np.eye(2)
+    first_term = sum(p[f] * q[f, s] * reward[s + 1] * (onehot[f] - p) for f in range(2) for s in range(2))
+    assert np.abs(first_term).max() > 0.01
+
+
+def test_draws_with_log_probabilities(dev):
+    """The draw that draw() makes, with the log-probability and the gradient that evaluate() gives for its paths."""
+    from src.gcn.algorithms.path_sampler import PathSampler
+    from src.gcn.hip import lib as L
+    B, V, C = 4, 14, 6
+    cap, comm = graphs(B, V, C)
+    kind = dict(temperature=1.3, top_p=0.9, entropy_epsilon=0.05)
+    y = torch.randn(B, V, V, C, device=dev, generator=torch.Generator(dev).manual_seed(8)).requires_grad_()
+    torch.manual_seed(21)
+    L.reseed()
+    paths, plen = PathSampler(y, cap, comm, **kind).draw()
+    L.reseed()
+    again, length, logp = PathSampler(y, cap, comm, **kind).draw_with_log_probs()
+    assert torch.equal(paths, again) and torch.equal(plen, length) and logp.shape == (B,)
+    _, want, _, _ = PathSampler(y, cap, comm, **kind).evaluate(paths, plen)
+    assert torch.equal(logp, want)
+    dy = torch.randn(B, device=dev)
+    got, base = torch.autograd.grad(logp, [y], dy)[0], torch.autograd.grad(want, [y], dy)[0]
+    assert float(base.abs().max()) > 0 and torch.equal(got, base)
