@@ -265,7 +265,9 @@ class ReinforcementLearningStrategy(BaseTrainingStrategy):
         params = [p for p in every if p.grad is not None]
         fused, stepped = isinstance(optimizer, FusedAdamW) and bool(params), False
         if fused and last_micro_step and self.grad_clip_max_norm > 0:
-            optimizer.step(max_grad_norm=self.grad_clip_max_norm)        # norm, clipping and update in the optimizer's launches
+            # norm, clipping and update in the optimizer's launches; its own limit holds too: the smaller of the two
+            limits = [self.grad_clip_max_norm] + ([] if optimizer.max_grad_norm is None else [optimizer.max_grad_norm])
+            optimizer.step(max_grad_norm=min(limits))
             total, stepped = optimizer.grad_norm.item(), True
         elif fused and len({p.dtype for p in params}) == 1:
             total = grad_norm([p.grad.contiguous() for p in params])[0].item()

@@ -314,3 +314,20 @@ def test_draws_with_log_probabilities(dev):
     dy = torch.randn(B, device=dev)
     got, base = torch.autograd.grad(logp, [y], dy)[0], torch.autograd.grad(want, [y], dy)[0]
     assert float(base.abs().max()) > 0 and torch.equal(got, base)
+
+
+@pytest.mark.parametrize("own, strategy, effective", [(0.01, 1.0, 0.01), (0.5, 0.02, 0.02), (0.01, 0.0, 0.01), (None, 0.02, 0.02), (None, 0.0, None)])
+def test_the_smaller_of_two_clipping_norms_holds(dev, own, strategy, effective):
+    """The optimizer's max_grad_norm and the strategy's: the first moment after one step is a tenth of the clipped gradient."""
+    extra = dict(rl_grad_clip_max_norm=strategy, **({} if own is None else dict(max_grad_norm=own)))
+    net, opt, strat, data = _strategy(dev, "adamw", **extra)
+    params = list(net.parameters())
+    grads = [torch.randn(p.shape, device=dev, generator=torch.Generator(dev).manual_seed(k)) for k, p in enumerate(params)]
+    norm = float(torch.sqrt(sum((g.double() ** 2).sum() for g in grads)))
+    assert strat.backward_step(sum((p * g).sum() for p, g in zip(params, grads)), opt, 1, 0)
+    assert abs(strat.grad_norm_history[-1] - norm) <= 2e-6 * norm
+    scale = 1.0 if effective is None else effective / (norm + 1e-6)
+    for p, g in zip(params, grads):
+        want = 0.1 * scale * g.double()
+        # (1 - b1), the coefficient and two products: 8 roundings
+        assert bool(((opt.state[p]["exp_avg"].double() - want).abs() <= 8 * U * want.abs() + 1e-44).all())
