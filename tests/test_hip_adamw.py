@@ -738,3 +738,27 @@ def test_parameters_that_skip_a_step_together_stay_one_list(dev, A, capturable):
     assert lists == [1, 1, 2, 2, 3]
     assert [int(opt.state[p]["step"]) for p in params] == [5] * 6 + [4] * 7 + [3] * 3
     assert len({id(opt.state[p]["step"]) for p in params}) == 3
+
+
+def test_8_bit_states_with_two_strides_a_workgroup(dev, A):
+    """Lists of more than 2^25 elements give a workgroup two strides: equal bits to the same tensors in calls of their own, which give one."""
+    sizes, gen = [12_000_001, 11_999_999, 10_002_177], torch.Generator(dev).manual_seed(12)
+    assert sum(sizes) > 1 << 25 and max(sizes) < 1 << 25
+    sets = []
+    for n in sizes:
+        p = torch.randn(n, device=dev, generator=gen)
+        m, v = 1e-2 * torch.randn(n, device=dev, generator=gen), 1e-2 * torch.rand(n, device=dev, generator=gen)
+        sets.append([p, torch.randn(n, device=dev, generator=gen) * 1e-2, *A.state8_encode(m), *A.state8_encode(v, never_zero=True)])
+    alone = [[t.clone() for t in s] for s in sets]
+    kind = dict(step=3, lr=1e-3, seed=77)
+
+    def step(group, first):
+        p, g, m, em, v, ev = (list(ts) for ts in zip(*group))
+        A.adamw_step_(p, g, m, v, exp_avg_exps=em, exp_avg_sq_exps=ev, first_tensor=first, **kind)
+    step(sets, 4)
+    for k, s in enumerate(alone):
+        before = s[0].clone()
+        step([s], 4 + k)
+        assert not torch.equal(before, s[0])
+    for a, b in zip(sets, alone):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

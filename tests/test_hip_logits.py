@@ -530,3 +530,50 @@ def test_out_that_overlaps_is_refused(dev):
             process_logits(x, out=out, **kind)
     assert torch.equal(process_logits(x, bias=buffer[2, 24:40], out=left), process_logits(x, bias=keep[2, 24:40].clone()))   # between out's rows
     assert torch.equal(buffer[:, 32:], keep[:, 32:])
+
+
+def vectorised(x, hist, lens, rho, tau, allowed, dy, bias_rows):
+    """dx, dbias and the magnitude of dbias' terms in double precision for logits [rows, vocab, inner], all rows at once."""
+    rows, vocab, _ = x.shape
+    seen = np.zeros((rows, vocab + 1), dtype=bool)
+    used = (np.arange(hist.shape[1]) < lens[:, None]) & (hist >= 0) & (hist < vocab)
+    seen[np.arange(rows)[:, None], np.where(used, hist, vocab)] = True
+    seen = seen[:, :vocab, None]
+    g = np.where(allowed[:, :, None], dy / tau[:, None, None], 0.0)
+    dx = g * np.where(seen, np.where(x > 0, 1 / rho[:, None, None], rho[:, None, None]), 1.0)
+    per = g.reshape(rows // bias_rows, bias_rows, vocab, -1)
+    return dx, per.sum((0, 3)), np.abs(per).sum((0, 3))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("bias_rows, times, vocab, inner, mask", [
+    (1024, 9, 14, 10, "bits"), (1024, 17, 6, 7, "bool"), (512, 20, 50, 100, "bits"), (1030, 8, 5, 3, None), (1024, 16, 3, 2, "bits"),
+    (1024, 33, 21, 1, "bits"), (1024, 70, 9, 1, "bool"), (512, 64, 4100, 1, None), (1025, 32, 8, 1, "bits"), (1024, 31, 40, 1, "bits"),
+    (1, 50000, 3, 1, "bits"), (4, 9000, 14, 10, "bits"), (3, 12000, 33, 1, None)])
+def test_gradient_over_many_rows_of_a_workgroup(dev, dtype, bias_rows, times, vocab, inner, mask):
+    """More than 1024 (bias row, range) pairs, so that a workgroup takes all `times` rows of a bias row, or so many rows that each of up to
+    1024 parts has dozens: several turns of 8 (scores) or 32 rows (tokens), the last one cut off, with histories that differ from row
+    to row; every row of dx, and dbias."""
+    from src.gcn.hip.logits import pack_mask, process_logits
+    rng, rows = np.random.default_rng(times), bias_rows * times
+    if rows * vocab * inner > 1 << 25 and dtype == torch.float32:
+        dtype = torch.float16                                                    # half the memory on the host, and the third type
+    x = torch.from_numpy(rng.standard_normal((rows, vocab, inner), dtype=np.float32)).to(dtype)
+    dy = torch.from_numpy(rng.standard_normal((rows, vocab, inner), dtype=np.float32)).to(dtype)
+    length = 12
+    hist, lens = rng.integers(-1, vocab + 1, (rows, length)), rng.integers(0, length + 1, rows)
+    rho, tau = rng.uniform(0.6, 1.7, rows).astype(np.float32), rng.uniform(0.5, 2.0, rows).astype(np.float32)
+    allowed = rng.random((rows, vocab)) < 0.8 if mask else np.ones((rows, vocab), dtype=bool)
+    put = lambda a: torch.from_numpy(a).to(dev)
+    shape = (rows, vocab) if inner == 1 else (rows, vocab, inner)
+    z = x.to(dev).view(shape).requires_grad_()
+    b = torch.zeros(bias_rows, vocab, device=dev, requires_grad=True)
+    kind = dict(dim=1, history=put(hist), history_lens=put(lens), repetition_penalty=put(rho), temperature=put(tau), masked_value=-1e4,
+                mask=None if mask is None else pack_mask(put(allowed)) if mask == "bits" else put(allowed))
+    got = torch.autograd.grad(process_logits(z, bias=b, **kind), [z, b], dy.to(dev).view(shape))
+    dx, db, size = vectorised(host(x), hist, lens, rho.astype(np.float64), tau.astype(np.float64), allowed, host(dy), bias_rows)
+    assert (np.abs(host(got[0], dx.shape) - dx) <= (4 * U + half_step(dtype)) * np.abs(dx) + 2.0 ** -25 * (dtype == torch.float16)).all()
+    assert (np.abs(host(got[1]) - db) <= (times * inner + 2) * U * size + 1e-44).all()
+    # without a bias: the rows are dealt to at most 1024 parts
+    (only,) = torch.autograd.grad(process_logits(z, **kind), [z], dy.to(dev).view(shape))
+    assert torch.equal(only, got[0])
