@@ -29,6 +29,12 @@ class FusedAdam(torch.optim.Optimizer):
             raise ValueError(f"Invalid weight_decay value: {weight_decay}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def load_state_dict(self, state_dict):
+        """As the base class, but codes of 8-bit moments (``FusedAdamW``) are refused: it would take them for moments."""
+        if any("exp_avg_exp" in st for st in state_dict["state"].values()):
+            raise ValueError("FusedAdam holds 32-bit moments, and the saved ones have 8 bits: load them into FusedAdamW, and its state_dict here")
+        super().load_state_dict(state_dict)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -198,3 +198,25 @@ def test_checkpoints_of_the_same_update_are_taken(source):
     for p, q in zip(mine, theirs):
         assert torch.equal(ours.state[p]["exp_avg"], opt.state[q]["exp_avg"]) and float(ours.state[p]["step"]) == 1
     assert ours.state[mine[0]]["step"] is ours.state[mine[1]]["step"]
+
+
+def test_fused_adam_refuses_8_bit_moments():
+    """Their codes are not moments; by way of a 32-bit FusedAdamW they are taken."""
+    from src.gcn.hip.fused_adam import FusedAdam
+    mine = [torch.nn.Parameter(torch.ones(300))]
+    narrow = A.FusedAdamW(mine, state_bits=8, min_8bit_numel=1, weight_decay=0.0)
+    moments = torch.linspace(-1, 1, 300)
+    st = {"step": torch.tensor(1.0)}
+    for key, x in (("exp_avg", moments), ("exp_avg_sq", moments.abs())):
+        st[key], st[key + "_exp"] = A.state8_encode(x, never_zero=key == "exp_avg_sq")
+    narrow.state[mine[0]] = st
+    other = [torch.nn.Parameter(torch.ones(300))]
+    adam = FusedAdam(other)
+    with pytest.raises(ValueError, match="8 bits"):
+        adam.load_state_dict(narrow.state_dict())
+    assert not adam.state
+    wide = A.FusedAdamW([torch.nn.Parameter(torch.ones(300))], weight_decay=0.0)
+    wide.load_state_dict(narrow.state_dict())
+    adam.load_state_dict(wide.state_dict())
+    # nearest code: off by half a step, 2^-4 of the value, or half of 2^-9 of the block's scale (the largest value is 1: 2^-7)
+    assert bool(((adam.state[other[0]]["exp_avg"] - moments).abs() <= (moments.abs() * 2.0 ** -4).clamp(min=2.0 ** -17)).all())
