@@ -20,7 +20,7 @@
 // Bound by memory: 28 bytes per element with fp32 states, 16 with 8-bit states (fp32: p and g in, p out; with 16-bit
 // parameters master and g in, master and p out).  120 M bf16 parameters with fp32 states: 618 us, 5.4 TB/s, which is what the best
 // copy reaches; 159 M with 8-bit states: 501 us, 5.1 TB/s, the vector units busy 67 % of the time (76 instructions an
-// element); 129 tensors of 174 k elements in all: 5.7 us, one launch, bound by its chain of dependent loads.
+// element); 127 tensors of 174 k elements in all: 5.6 us, one launch, bound by its chain of dependent loads.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -58,6 +58,8 @@ struct AdamwHyper {
     uint32_t pad;
 };
 
+// A published mixing function of 32-bit integers (C. Wellons, 2018; its shifts and multipliers come from a search for low bias).  The
+// hash's other constants are published ones too: 2^32 over the golden ratio, and two multipliers of A. Appleby's (2011).
 __device__ __host__ inline uint32_t opt_mix(uint32_t x) {
     x ^= x >> 16; x *= 0x7feb352dU; x ^= x >> 15; x *= 0x846ca68bU; x ^= x >> 16;
     return x;

@@ -74,7 +74,8 @@ def adamw_advance_(step, hyper, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_deca
 
 def grad_norm(grads, *, max_norm=None, grad_scale=None):
     """(norm, coefficient): the 2-norm of all gradients together, times grad_scale, and min(1, max_norm / (norm + 1e-6)) or None
-    without max_norm, as scalars on the device.  The gradients are of one type and on one GPU and are not changed."""
+    without max_norm, as scalars on the device.  The gradients are of one type and on one GPU and are not changed; autograd takes the
+    results as constants."""
     return L.binding().grad_norm(grads, max_norm, grad_scale)
 
 
